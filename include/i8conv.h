@@ -228,6 +228,126 @@ int i8conv_pack_vect_c(const int8_t *src, int8_t *dst, int n, int h, int w,
 int i8conv_unpack_vect_c(const int8_t *src, int8_t *dst, int n, int h, int w,
                          int c, int vect, void *stream);
 
+/* ---- int8 linear layers (no counterpart in the reference) --------------- */
+
+/* The matrix products of language models on the lab's int8 arithmetic:
+ * activations quantized to int8 row by row, int8 weights with a scale per
+ * output channel, exact int32 sums (inputs < 2^17), and the rest in 32-bit
+ * floating point, rounded to the output's type once:
+ *   v[m][n] = (sum_k code[m][k] * w[n][k]) * row_scale[m] * weight_scale[n]
+ *             + bias[n]
+ *   y[m][n] = act(v[m][n]) + residual[m][n]
+ * Gated layers have 2 * outputs weight rows, scales and biases, the activated
+ * half first:
+ *   y[m][n] = act(v[m][n]) * v[m][outputs + n] + residual[m][n]
+ * Layers of experts have one such weight matrix per expert, and rows sorted
+ * by expert (i8conv_launch_route).
+ *
+ * Launches are asynchronous on `stream` and allocate nothing; results are
+ * repeatable bit for bit.  The output overlaps no other tensor, except that
+ * the residual may be the output itself (the same rows and stride). */
+
+typedef enum i8conv_type {
+  I8CONV_INT8 = 0,
+  I8CONV_BF16 = 1,
+  I8CONV_FP16 = 2,
+  I8CONV_FP32 = 3
+} i8conv_type;
+
+typedef enum i8conv_activation {
+  I8CONV_ACT_NONE = 0,
+  I8CONV_ACT_RELU = 1,
+  I8CONV_ACT_GELU = 2,      /* v (1 + erf(v / sqrt 2)) / 2 */
+  I8CONV_ACT_GELU_TANH = 3, /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
+  I8CONV_ACT_SILU = 4       /* v / (1 + exp(-v)) */
+} i8conv_activation;
+
+/* A linear layer.  `rows` may be 0 (nothing is launched).  inputs % 16 == 0
+ * and < 2^17; the weights of one matrix (outputs, or 2 * outputs where gated,
+ * times inputs) below 2^31 bytes.  Strides are elements between rows, 0 for
+ * packed rows; that of an int8 input is a multiple of 16 below 2^23. */
+typedef struct i8conv_linear_shape {
+  int32_t rows;            /* rows of the input (tokens) */
+  int32_t inputs, outputs; /* values of a row */
+  int32_t input_type;      /* i8conv_type; the output's type is no INT8 */
+  int32_t output_type;     /* also the residual's */
+  int32_t activation;      /* i8conv_activation */
+  int32_t gated;           /* 0 or 1 */
+  int32_t experts;         /* 0: a dense layer; at most 4096 */
+  int32_t routed;          /* by expert: rows of the output, at most */
+  int64_t input_stride, output_stride, residual_stride;
+} i8conv_linear_shape;
+
+/* Device memory that a launch of `shape` needs, 256-byte aligned: the codes and
+ * scales of an input that is quantized on the way.  0 for a bad shape. */
+size_t i8conv_linear_workspace_bytes(const i8conv_linear_shape *shape);
+
+/* A dense layer.  `input_scale` (rows floats) belongs to an int8 input and is
+ * NULL with any other, whose rows are quantized as by i8conv_quantize_rows.
+ * `bias` (floats) and `residual` may be NULL.  weight [outputs or 2 outputs]
+ * [inputs] and an int8 input are 16-byte aligned, other tensors to their
+ * elements (16-byte alignment and outputs % 4 == 0 are faster). */
+int i8conv_launch_linear(const i8conv_linear_shape *shape, const void *input,
+                         const float *input_scale, const int8_t *weight,
+                         const float *weight_scale, const float *bias,
+                         const void *residual, void *output, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+/* A layer of experts: output row r, offsets[e] <= r < offsets[e + 1], is input
+ * row sources[r] (r itself where `sources` is NULL, and then rows >= routed)
+ * through expert e's weights, scales and bias ([experts][outputs or 2
+ * outputs]...).  `offsets` (experts + 1, rising from 0) and `sources` are device
+ * arrays, as i8conv_launch_route writes them; output rows at or past
+ * offsets[experts] are left as they are.  A source outside [0, rows) reads as a
+ * row of zeros.  With `sources` the int8 codes of the input stay below 2^31
+ * bytes. */
+int i8conv_launch_expert_linear(const i8conv_linear_shape *shape, const void *input,
+                                const float *input_scale, const int8_t *weight,
+                                const float *weight_scale, const float *bias,
+                                const int32_t *offsets, const int32_t *sources,
+                                void *output, void *workspace,
+                                size_t workspace_bytes, void *stream);
+
+/* Rows to int8 codes and their scales, with a = max |x[k]| of a row:
+ *   code[k] = rint(127 x[k] / a) (half to even),  scale = a / 127.
+ * A row with a < 2^-100 gives zeros and scale 0, a row with an infinity or NaN
+ * zeros and scale NaN.  inputs % 16 == 0; codes are packed, 16-byte aligned. */
+int i8conv_quantize_rows(const void *input, int type, int32_t rows, int32_t inputs,
+                         int64_t input_stride, int8_t *codes, float *scales,
+                         void *stream);
+
+/* tokens x choices expert ids, below 2^31 in all; at most 4096 experts. */
+typedef struct i8conv_route_shape {
+  int32_t tokens, choices, experts;
+} i8conv_route_shape;
+
+/* Device memory that a launch of `shape` needs, 256-byte aligned. */
+size_t i8conv_route_workspace_bytes(const i8conv_route_shape *shape);
+
+/* The stable sort of the choices by expert: ids [tokens][choices] to
+ *   offsets [experts + 1]     where each expert's rows begin, and their end,
+ *   sources [tokens * choices]  the token of each row; -1 past the last row,
+ *   places  [tokens][choices]   the row of each choice; -1 for an id outside
+ *                               [0, experts), which gets no row. */
+int i8conv_launch_route(const i8conv_route_shape *shape, const int32_t *ids,
+                        int32_t *offsets, int32_t *sources, int32_t *places,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
+/* Packed rows of `outputs` values; neither type is INT8. */
+typedef struct i8conv_combine_shape {
+  int32_t tokens, choices, outputs;
+  int32_t input_type, output_type;
+} i8conv_combine_shape;
+
+/* A token's weighted sum of its experts' rows, in the order of its choices and
+ * in 32-bit floating point:
+ *   y[t] = residual[t] + sum_c weights[t][c] * input[places[t][c]]
+ * with places outside [0, tokens * choices) left out.  `residual` (the
+ * output's type) may be NULL or the output. */
+int i8conv_launch_combine(const i8conv_combine_shape *shape, const void *input,
+                          const int32_t *places, const float *weights,
+                          const void *residual, void *output, void *stream);
+
 /* ---- thin HIP runtime layer used by the host driver -------------------- */
 
 /* DeviceBuffer (conv_lab.cu:24-37) as C calls. */

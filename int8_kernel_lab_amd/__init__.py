@@ -15,6 +15,10 @@ plus the candidates the reference does not have (``halo``, ``splitk``), the
 dispatch policy and a one-call ``conv2d``.  Tensors are NHWC int8 input, KRSC
 int8 filter, K int32 bias, NHWK int32 output.  Every GPU call goes through
 libi8conv.so; nothing here computes a convolution on the CPU.
+
+The int8 linear layers of language models (``LinearShape``, ``launch_linear``,
+``launch_expert_linear`` and what feeds and follows them) have no counterpart
+in the reference.
 """
 from __future__ import annotations
 
@@ -39,6 +43,9 @@ __all__ = [
     "conv2d_requant", "measure_requant", "nchw_to_nhwc", "nhwc_to_nchw", "nhwk_to_nkhw",
     "pack_vect_c", "unpack_vect_c", "measure_graph", "measure_store_floor", "measure_lds_probe", "wait_expired", "launch_noalloc",
     "set_wait_spin_limit", "wait_spin_limit", "DEFAULT_WAIT_SPIN_LIMIT",
+    "LinearShape", "RouteShape", "CombineShape", "linear_workspace_bytes", "launch_linear",
+    "launch_expert_linear", "quantize_rows", "route_workspace_bytes", "launch_route",
+    "launch_combine",
 ]
 
 KERNELS = ("generic", "strip", "halo", "splitk")
@@ -607,3 +614,157 @@ def pack_vect_c(src, dst, n: int, h: int, w: int, c: int, vect: int = 32, stream
 def unpack_vect_c(src, dst, n: int, h: int, w: int, c: int, vect: int = 32, stream=None) -> None:
     check(lib().i8conv_unpack_vect_c(_ptr(src), _ptr(dst), n, h, w, c, vect, _ptr(stream)),
           "unpack_vect_c")
+
+
+# ---- int8 linear layers (no reference counterpart) --------------------------
+
+TYPES = {"int8": 0, "bf16": 1, "fp16": 2, "fp32": 3}
+TYPE_BYTES = {"int8": 1, "bf16": 2, "fp16": 2, "fp32": 4}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _code(table: Dict[str, int], name: str, what: str) -> int:
+    if name not in table:
+        raise ValueError(f"unknown {what} {name!r}; known: {tuple(table)}")
+    return table[name]
+
+
+class _Described(_CRefSlot):
+    """A shape whose C struct is built once (see ConvShape._c_ref)."""
+
+    __slots__ = ()
+
+    def _c_ref(self):
+        ref = getattr(self, "_ref", None)
+        if ref is None:
+            ref = ctypes.byref(self.c_struct())
+            object.__setattr__(self, "_ref", ref)
+        return ref
+
+    def __getstate__(self):  # not the C struct: it points into this process
+        return self.__dict__
+
+
+@dataclass(frozen=True)
+class LinearShape(_Described):
+    """An int8 linear layer (i8conv_linear_shape), dense (experts == 0) or by
+    expert.  Types and activations by name; strides in elements, 0 if packed."""
+
+    rows: int
+    inputs: int
+    outputs: int
+    input_type: str = "bf16"
+    output_type: str = "bf16"
+    activation: str = "none"
+    gated: bool = False
+    experts: int = 0
+    routed: int = 0
+    input_stride: int = 0
+    output_stride: int = 0
+    residual_stride: int = 0
+
+    def c_struct(self) -> _lib.CLinearShape:
+        return _lib.CLinearShape(
+            int(self.rows), int(self.inputs), int(self.outputs),
+            _code(TYPES, self.input_type, "type"), _code(TYPES, self.output_type, "type"),
+            _code(ACTIVATIONS, self.activation, "activation"), int(bool(self.gated)),
+            int(self.experts), int(self.routed), int(self.input_stride),
+            int(self.output_stride), int(self.residual_stride))
+
+    @property
+    def weight_rows(self) -> int:
+        """Rows of one weight matrix: the gate's and the other half's."""
+        return 2 * self.outputs if self.gated else self.outputs
+
+    def ops(self) -> int:
+        """2 * rows * weight rows * inputs (by expert: of every routed row)."""
+        return 2 * (self.routed if self.experts else self.rows) * self.weight_rows * self.inputs
+
+
+@dataclass(frozen=True)
+class RouteShape(_Described):
+    """tokens x choices of `experts` experts (i8conv_route_shape)."""
+
+    tokens: int
+    choices: int
+    experts: int
+
+    def c_struct(self) -> _lib.CRouteShape:
+        return _lib.CRouteShape(int(self.tokens), int(self.choices), int(self.experts))
+
+
+@dataclass(frozen=True)
+class CombineShape(_Described):
+    """tokens x choices rows of `outputs` values (i8conv_combine_shape)."""
+
+    tokens: int
+    choices: int
+    outputs: int
+    input_type: str = "bf16"
+    output_type: str = "bf16"
+
+    def c_struct(self) -> _lib.CCombineShape:
+        return _lib.CCombineShape(int(self.tokens), int(self.choices), int(self.outputs),
+                                  _code(TYPES, self.input_type, "type"),
+                                  _code(TYPES, self.output_type, "type"))
+
+
+def linear_workspace_bytes(shape: LinearShape) -> int:
+    return int(lib().i8conv_linear_workspace_bytes(shape._c_ref()))
+
+
+def launch_linear(shape: LinearShape, input, input_scale, weight, weight_scale, bias, residual,
+                  output, workspace=None, workspace_nbytes: int = 0, stream=None) -> None:
+    """act(x w^T * scales + bias) [* gated half] + residual, asynchronous
+    (i8conv_launch_linear).  input_scale only with an int8 input; bias and
+    residual may be None."""
+    if isinstance(workspace, DeviceBuffer) and not workspace_nbytes:
+        workspace_nbytes = workspace.nbytes
+    check(lib().i8conv_launch_linear(shape._c_ref(), _ptr(input), _ptr(input_scale), _ptr(weight),
+                                     _ptr(weight_scale), _ptr(bias), _ptr(residual), _ptr(output),
+                                     _ptr(workspace), int(workspace_nbytes), _ptr(stream)),
+          "launch_linear")
+
+
+def launch_expert_linear(shape: LinearShape, input, input_scale, weight, weight_scale, bias,
+                         offsets, sources, output, workspace=None, workspace_nbytes: int = 0,
+                         stream=None) -> None:
+    """The same with one weight matrix per expert, over rows sorted by expert
+    (i8conv_launch_expert_linear); offsets and sources as launch_route writes
+    them, sources None for rows that lie in that order."""
+    if isinstance(workspace, DeviceBuffer) and not workspace_nbytes:
+        workspace_nbytes = workspace.nbytes
+    check(lib().i8conv_launch_expert_linear(
+        shape._c_ref(), _ptr(input), _ptr(input_scale), _ptr(weight), _ptr(weight_scale),
+        _ptr(bias), _ptr(offsets), _ptr(sources), _ptr(output), _ptr(workspace),
+        int(workspace_nbytes), _ptr(stream)), "launch_expert_linear")
+
+
+def quantize_rows(input, input_type: str, rows: int, inputs: int, codes, scales,
+                  input_stride: int = 0, stream=None) -> None:
+    """Rows to int8 codes and one scale each (i8conv_quantize_rows)."""
+    check(lib().i8conv_quantize_rows(_ptr(input), _code(TYPES, input_type, "type"), int(rows),
+                                     int(inputs), int(input_stride), _ptr(codes), _ptr(scales),
+                                     _ptr(stream)), "quantize_rows")
+
+
+def route_workspace_bytes(shape: RouteShape) -> int:
+    return int(lib().i8conv_route_workspace_bytes(shape._c_ref()))
+
+
+def launch_route(shape: RouteShape, ids, offsets, sources, places, workspace=None,
+                 workspace_nbytes: int = 0, stream=None) -> None:
+    """The stable sort of the tokens' choices by expert (i8conv_launch_route)."""
+    if isinstance(workspace, DeviceBuffer) and not workspace_nbytes:
+        workspace_nbytes = workspace.nbytes
+    check(lib().i8conv_launch_route(shape._c_ref(), _ptr(ids), _ptr(offsets), _ptr(sources),
+                                    _ptr(places), _ptr(workspace), int(workspace_nbytes),
+                                    _ptr(stream)), "launch_route")
+
+
+def launch_combine(shape: CombineShape, input, places, weights, residual, output,
+                   stream=None) -> None:
+    """Each token's weighted sum of its experts' rows (i8conv_launch_combine)."""
+    check(lib().i8conv_launch_combine(shape._c_ref(), _ptr(input), _ptr(places), _ptr(weights),
+                                      _ptr(residual), _ptr(output), _ptr(stream)),
+          "launch_combine")

@@ -52,6 +52,28 @@ class CGraphTiming(ctypes.Structure):
                 ("stream_ms", c_float), ("kernel_ms", c_float)]
 
 
+class CLinearShape(ctypes.Structure):
+    """struct i8conv_linear_shape."""
+
+    _fields_ = [(name, c_int32) for name in (
+        "rows", "inputs", "outputs", "input_type", "output_type", "activation", "gated",
+        "experts", "routed")] + [(name, c_int64) for name in (
+            "input_stride", "output_stride", "residual_stride")]
+
+
+class CRouteShape(ctypes.Structure):
+    """struct i8conv_route_shape."""
+
+    _fields_ = [(name, c_int32) for name in ("tokens", "choices", "experts")]
+
+
+class CCombineShape(ctypes.Structure):
+    """struct i8conv_combine_shape."""
+
+    _fields_ = [(name, c_int32) for name in ("tokens", "choices", "outputs", "input_type",
+                                             "output_type")]
+
+
 # name -> (restype, argtypes); every symbol include/i8conv.h declares.
 SIGNATURES = {
     "i8conv_derive": (c_int, [POINTER(CShape), POINTER(CGeometry)]),
@@ -91,6 +113,17 @@ SIGNATURES = {
                                    c_void_p]),
     "i8conv_unpack_vect_c": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                      c_void_p]),
+    "i8conv_linear_workspace_bytes": (c_size_t, [POINTER(CLinearShape)]),
+    "i8conv_launch_linear": (c_int, [POINTER(CLinearShape)] + [c_void_p] * 8 +
+                             [c_size_t, c_void_p]),
+    "i8conv_launch_expert_linear": (c_int, [POINTER(CLinearShape)] + [c_void_p] * 9 +
+                                    [c_size_t, c_void_p]),
+    "i8conv_quantize_rows": (c_int, [c_void_p, c_int, c_int32, c_int32, c_int64, c_void_p,
+                                     c_void_p, c_void_p]),
+    "i8conv_route_workspace_bytes": (c_size_t, [POINTER(CRouteShape)]),
+    "i8conv_launch_route": (c_int, [POINTER(CRouteShape)] + [c_void_p] * 5 +
+                            [c_size_t, c_void_p]),
+    "i8conv_launch_combine": (c_int, [POINTER(CCombineShape)] + [c_void_p] * 6),
     "i8conv_device_count": (c_int, [POINTER(c_int)]),
     "i8conv_set_device": (c_int, [c_int]),
     "i8conv_device_alloc": (c_int, [POINTER(c_void_p), c_size_t]),

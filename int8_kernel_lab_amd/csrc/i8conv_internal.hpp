@@ -216,6 +216,17 @@ int launch_transpose(const void *src, void *dst, int64_t batch, int rows, int co
                      void *stream);
 int launch_pack_vect(const int8_t *src, int8_t *dst, int n, int h, int w, int c, int vect,
                      bool unpack, void *stream);
+// kernel_quantize.hip, kernel_linear.hip, kernel_experts.hip: the int8 linear
+// layers' launchers, on checked arguments (linear_capi.hip).
+struct LinearArgs;
+int launch_quantize(const void *x, int type, int64_t ldx, int rows, int k, int8_t *codes,
+                    float *scales, void *stream);
+int launch_linear_tiles(const LinearArgs &a, bool gated, void *stream);
+int launch_route(const int32_t *ids, int tokens, int choices, int experts, int32_t *offsets,
+                 int32_t *sources, int32_t *places, void *stream);
+int launch_combine(const void *x, int in_type, const int32_t *places, const float *weights,
+                   const void *residual, void *y, int out_type, int tokens, int choices, int n,
+                   void *stream);
 // q == nullptr: int32 output to a.y; else the requantized int8 output to
 // q->y, computed in the kernel's epilogue (a.y unused)
 int launch_rowpass(const ConvArgs &a, const PatchPlan &p, void *stream,

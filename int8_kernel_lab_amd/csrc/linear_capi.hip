@@ -1,0 +1,242 @@
+// The C ABI of the int8 linear layers: argument checks, workspace layout and
+// which kernels a launch runs.
+#include <hip/hip_runtime.h>
+
+#include <string>
+
+#include "i8conv_internal.hpp"
+#include "linear_common.hpp"
+
+namespace i8conv {
+namespace {
+
+constexpr int kMaxExperts = 4096;
+constexpr int64_t kMaxBytes = (int64_t(1) << 31) - 1;
+
+bool aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
+int fail(int status, const char *what) {
+  set_error(what);
+  return status;
+}
+
+bool float_type(int t) { return t == I8CONV_BF16 || t == I8CONV_FP16 || t == I8CONV_FP32; }
+
+int check_shape(const i8conv_linear_shape *s) {
+  if (!s) return fail(I8CONV_BAD_ARGUMENT, "null shape");
+  if (s->rows < 0 || s->outputs < 1 || s->experts < 0 || s->routed < 0 || s->experts > kMaxExperts)
+    return fail(I8CONV_BAD_SHAPE, "linear: rows, routed >= 0, outputs >= 1 and 0 <= experts <= 4096");
+  if (s->inputs < 16 || s->inputs % 16 != 0 || s->inputs >= 1 << 17)
+    return fail(I8CONV_BAD_SHAPE, "linear: inputs must be a multiple of 16 below 2^17");
+  if (s->input_type != I8CONV_INT8 && !float_type(s->input_type))
+    return fail(I8CONV_BAD_SHAPE, "linear: unknown input type");
+  if (!float_type(s->output_type))
+    return fail(I8CONV_BAD_SHAPE, "linear: the output is bf16, fp16 or fp32");
+  if (s->activation < I8CONV_ACT_NONE || s->activation > I8CONV_ACT_SILU)
+    return fail(I8CONV_BAD_SHAPE, "linear: unknown activation");
+  if (s->gated != 0 && s->gated != 1) return fail(I8CONV_BAD_SHAPE, "linear: gated is 0 or 1");
+  if (s->experts == 0 && s->routed != 0)
+    return fail(I8CONV_BAD_SHAPE, "linear: routed rows belong to a layer of experts");
+  if ((int64_t(s->outputs) << s->gated) * s->inputs > kMaxBytes)
+    return fail(I8CONV_BAD_SHAPE, "linear: a weight matrix above 2^31-1 bytes");
+  if ((s->input_stride != 0 && s->input_stride < s->inputs) ||
+      (s->output_stride != 0 && s->output_stride < s->outputs) ||
+      (s->residual_stride != 0 && s->residual_stride < s->outputs))
+    return fail(I8CONV_BAD_SHAPE, "linear: a stride below the row's length");
+  if (s->input_type == I8CONV_INT8 && (s->input_stride % 16 != 0 || s->input_stride >= 1 << 23))
+    return fail(I8CONV_BAD_SHAPE, "linear: the stride of int8 rows is a multiple of 16 below 2^23");
+  return I8CONV_OK;
+}
+
+// Workspace: codes [rows][inputs], then scales [rows].
+size_t codes_bytes(const i8conv_linear_shape &s) { return align256(size_t(s.rows) * s.inputs); }
+
+size_t workspace_bytes(const i8conv_linear_shape &s) {
+  if (s.input_type == I8CONV_INT8) return 0;
+  return codes_bytes(s) + align256(size_t(s.rows) * 4);
+}
+
+int check_tensors(const i8conv_linear_shape &s, const void *input, const float *input_scale,
+                  const int8_t *weight, const float *weight_scale, const float *bias,
+                  const void *residual, const void *output, const void *workspace,
+                  size_t workspace_size) {
+  if (!input || !weight || !weight_scale || !output)
+    return fail(I8CONV_BAD_ARGUMENT, "linear: null tensor pointer");
+  const bool codes = s.input_type == I8CONV_INT8;
+  if (codes != (input_scale != nullptr))
+    return fail(I8CONV_BAD_ARGUMENT, "linear: row scales belong to an int8 input, and only to one");
+  if (!aligned(weight, 16) || (codes && !aligned(input, 16)))
+    return fail(I8CONV_BAD_ARGUMENT, "linear: weights and int8 inputs must be 16-byte aligned");
+  if (!aligned(input, type_size(s.input_type)) || !aligned(output, type_size(s.output_type)) ||
+      !aligned(residual, type_size(s.output_type)) || !aligned(input_scale, 4) ||
+      !aligned(weight_scale, 4) || !aligned(bias, 4))
+    return fail(I8CONV_BAD_ARGUMENT, "linear: a tensor is not aligned to its elements");
+  const size_t need = workspace_bytes(s);
+  if (need && (!workspace || workspace_size < need || !aligned(workspace, 256))) {
+    set_error("linear: needs a 256-byte aligned workspace of " + std::to_string(need) + " bytes");
+    return I8CONV_WORKSPACE_TOO_SMALL;
+  }
+  return I8CONV_OK;
+}
+
+int run(const i8conv_linear_shape &s, const void *input, const float *input_scale,
+        const int8_t *weight, const float *weight_scale, const float *bias, const void *residual,
+        const int32_t *offsets, const int32_t *sources, void *output, void *workspace,
+        void *stream) {
+  LinearArgs a{};
+  const int size = type_size(s.output_type);
+  a.w = weight;
+  a.ws = weight_scale;
+  a.bias = bias;
+  a.residual = residual;
+  a.y = output;
+  a.offsets = offsets;
+  a.sources = sources;
+  a.ldx = s.input_stride ? s.input_stride : s.inputs;
+  a.ldy = s.output_stride ? s.output_stride : s.outputs;
+  a.ldr = s.residual_stride ? s.residual_stride : s.outputs;
+  a.x_rows = s.rows;
+  a.rows = s.experts ? s.routed : s.rows;
+  a.k = s.inputs;
+  a.n = s.outputs;
+  a.wide = s.outputs << s.gated;
+  a.experts = s.experts;
+  a.activation = s.activation;
+  a.out_type = s.output_type;
+  a.vec = linear_vec_ok(output, a.ldy, a.n, size) &&
+          (!residual || linear_vec_ok(residual, a.ldr, a.n, size));
+  if (s.input_type == I8CONV_INT8) {
+    a.x = static_cast<const int8_t *>(input);
+    a.xs = input_scale;
+  } else {
+    int8_t *const codes = static_cast<int8_t *>(workspace);
+    float *const scales = reinterpret_cast<float *>(codes + codes_bytes(s));
+    const int rc = launch_quantize(input, s.input_type, a.ldx, s.rows, s.inputs, codes, scales, stream);
+    if (rc != I8CONV_OK) return rc;
+    a.x = codes;
+    a.xs = scales;
+    a.ldx = s.inputs;
+  }
+  return launch_linear_tiles(a, s.gated != 0, stream);
+}
+
+int check_route(const i8conv_route_shape *s) {
+  if (!s) return fail(I8CONV_BAD_ARGUMENT, "null shape");
+  if (s->tokens < 0 || s->choices < 1 || s->experts < 1 || s->experts > kMaxExperts ||
+      int64_t(s->tokens) * s->choices > kMaxBytes)
+    return fail(I8CONV_BAD_SHAPE,
+                "route: tokens >= 0, choices >= 1, 1 <= experts <= 4096 and tokens * choices < 2^31");
+  return I8CONV_OK;
+}
+
+}  // namespace
+}  // namespace i8conv
+
+using namespace i8conv;
+
+extern "C" {
+
+size_t i8conv_linear_workspace_bytes(const i8conv_linear_shape *shape) {
+  return check_shape(shape) == I8CONV_OK ? workspace_bytes(*shape) : 0;
+}
+
+int i8conv_launch_linear(const i8conv_linear_shape *shape, const void *input,
+                         const float *input_scale, const int8_t *weight, const float *weight_scale,
+                         const float *bias, const void *residual, void *output, void *workspace,
+                         size_t workspace_size, void *stream) {
+  int rc = check_shape(shape);
+  if (rc != I8CONV_OK) return rc;
+  if (shape->experts)
+    return fail(I8CONV_BAD_SHAPE, "linear: a layer of experts goes through launch_expert_linear");
+  if (shape->rows == 0) return I8CONV_OK;
+  rc = check_tensors(*shape, input, input_scale, weight, weight_scale, bias, residual, output,
+                     workspace, workspace_size);
+  if (rc != I8CONV_OK) return rc;
+  return run(*shape, input, input_scale, weight, weight_scale, bias, residual, nullptr, nullptr,
+             output, workspace, stream);
+}
+
+int i8conv_launch_expert_linear(const i8conv_linear_shape *shape, const void *input,
+                                const float *input_scale, const int8_t *weight,
+                                const float *weight_scale, const float *bias,
+                                const int32_t *offsets, const int32_t *sources, void *output,
+                                void *workspace, size_t workspace_size, void *stream) {
+  int rc = check_shape(shape);
+  if (rc != I8CONV_OK) return rc;
+  if (!shape->experts) return fail(I8CONV_BAD_SHAPE, "expert linear: experts must be at least 1");
+  if (!sources && shape->rows < shape->routed)
+    return fail(I8CONV_BAD_SHAPE, "expert linear: without sources rows must be at least routed");
+  const int64_t ld = shape->input_type == I8CONV_INT8 && shape->input_stride ? shape->input_stride
+                                                                            : shape->inputs;
+  if (sources && int64_t(shape->rows) * ld > kMaxBytes)
+    return fail(I8CONV_BAD_SHAPE, "expert linear: gathered codes above 2^31-1 bytes");
+  if (shape->routed == 0 || shape->rows == 0) return I8CONV_OK;
+  rc = check_tensors(*shape, input, input_scale, weight, weight_scale, bias, nullptr, output,
+                     workspace, workspace_size);
+  if (rc != I8CONV_OK) return rc;
+  if (!offsets || !aligned(offsets, 4) || !aligned(sources, 4))
+    return fail(I8CONV_BAD_ARGUMENT, "expert linear: offsets are needed, 4-byte aligned like sources");
+  return run(*shape, input, input_scale, weight, weight_scale, bias, nullptr, offsets, sources,
+             output, workspace, stream);
+}
+
+int i8conv_quantize_rows(const void *input, int type, int32_t rows, int32_t inputs,
+                         int64_t input_stride, int8_t *codes, float *scales, void *stream) {
+  if (!float_type(type) || rows < 0 || inputs < 16 || inputs % 16 != 0 ||
+      (input_stride != 0 && input_stride < inputs))
+    return fail(I8CONV_BAD_ARGUMENT,
+                "quantize_rows: a floating type, rows >= 0, inputs a positive multiple of 16 and a "
+                "stride of 0 or at least inputs");
+  if (rows == 0) return I8CONV_OK;
+  if (!input || !codes || !scales)
+    return fail(I8CONV_BAD_ARGUMENT, "quantize_rows: null tensor pointer");
+  if (!aligned(input, type_size(type)) || !aligned(codes, 16) || !aligned(scales, 4))
+    return fail(I8CONV_BAD_ARGUMENT,
+                "quantize_rows: codes must be 16-byte aligned, other tensors to their elements");
+  return launch_quantize(input, type, input_stride ? input_stride : inputs, rows, inputs, codes,
+                         scales, stream);
+}
+
+size_t i8conv_route_workspace_bytes(const i8conv_route_shape *shape) {
+  (void)shape;
+  return 0;
+}
+
+int i8conv_launch_route(const i8conv_route_shape *shape, const int32_t *ids, int32_t *offsets,
+                        int32_t *sources, int32_t *places, void *workspace, size_t workspace_size,
+                        void *stream) {
+  const int rc = check_route(shape);
+  if (rc != I8CONV_OK) return rc;
+  (void)workspace;
+  (void)workspace_size;
+  if (!offsets || (shape->tokens > 0 && (!ids || !sources || !places)))
+    return fail(I8CONV_BAD_ARGUMENT, "route: null tensor pointer");
+  if (!aligned(ids, 4) || !aligned(offsets, 4) || !aligned(sources, 4) || !aligned(places, 4))
+    return fail(I8CONV_BAD_ARGUMENT, "route: tensors must be 4-byte aligned");
+  return launch_route(ids, shape->tokens, shape->choices, shape->experts, offsets, sources, places,
+                      stream);
+}
+
+int i8conv_launch_combine(const i8conv_combine_shape *shape, const void *input,
+                          const int32_t *places, const float *weights, const void *residual,
+                          void *output, void *stream) {
+  if (!shape) return fail(I8CONV_BAD_ARGUMENT, "null shape");
+  if (shape->tokens < 0 || shape->choices < 1 || shape->outputs < 1 ||
+      int64_t(shape->tokens) * shape->choices > kMaxBytes)
+    return fail(I8CONV_BAD_SHAPE,
+                "combine: tokens >= 0, choices >= 1, outputs >= 1 and tokens * choices < 2^31");
+  if (!float_type(shape->input_type) || !float_type(shape->output_type))
+    return fail(I8CONV_BAD_SHAPE, "combine: types are bf16, fp16 or fp32");
+  if (shape->tokens == 0) return I8CONV_OK;
+  if (!input || !places || !weights || !output)
+    return fail(I8CONV_BAD_ARGUMENT, "combine: null tensor pointer");
+  const int out = type_size(shape->output_type);
+  if (!aligned(input, type_size(shape->input_type)) || !aligned(output, out) ||
+      !aligned(residual, out) || !aligned(places, 4) || !aligned(weights, 4))
+    return fail(I8CONV_BAD_ARGUMENT, "combine: a tensor is not aligned to its elements");
+  return launch_combine(input, shape->input_type, places, weights, residual, output,
+                        shape->output_type, shape->tokens, shape->choices, shape->outputs, stream);
+}
+
+}  // extern "C"

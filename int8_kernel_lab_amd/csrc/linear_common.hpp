@@ -1,0 +1,129 @@
+// What the int8 linear layers' kernels share: their arguments, the value
+// types, and the arithmetic after the integer sums,
+//   y = act(sum * row scale * channel scale + bias) [* gated half] + residual,
+// in 32-bit floating point and rounded to the output's type once.
+#pragma once
+
+#include <stdint.h>
+
+#include "i8conv.h"
+#include "i8conv_device.hpp"
+
+namespace i8conv {
+
+// Arguments of a linear layer's product, dense or by expert.
+struct LinearArgs {
+  const int8_t *x;      // codes [x_rows][ldx]
+  const float *xs;      // [x_rows]
+  const int8_t *w;      // [experts or 1][wide][k]
+  const float *ws;      // [experts or 1][wide]
+  const float *bias;    // [experts or 1][wide] or null
+  const void *residual; // [rows][ldr], the output's type, or null
+  void *y;              // [rows][ldy]
+  const int32_t *offsets;  // by expert: [experts + 1], else null
+  const int32_t *sources;  // by expert: x row of each row, or null
+  int64_t ldx, ldy, ldr;   // elements
+  int x_rows, rows;        // rows of x; rows of y (by expert: their upper bound)
+  int k, n, wide;          // wide = n, or 2 n where gated
+  int experts;             // 0: dense
+  int activation, out_type;
+  bool vec;  // four consecutive outputs may move at once (see linear_vec_ok)
+};
+
+// Whether rows of n values of `size` bytes at base + row * ld may be moved four
+// at a time.
+inline bool linear_vec_ok(const void *base, int64_t ld, int n, int size) {
+  return n % 4 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(base) & (4 * size - 1)) == 0;
+}
+
+I8_HD inline int type_size(int type) {
+  return type == I8CONV_INT8 ? 1 : type == I8CONV_FP32 ? 4 : 2;
+}
+
+#if defined(__HIPCC__)
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float bits_f32(uint32_t b) { return __builtin_bit_cast(float, b); }
+__device__ __forceinline__ uint32_t f32_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
+
+__device__ __forceinline__ uint16_t to_bf16(float f) {
+  return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f));  // to nearest even
+}
+__device__ __forceinline__ uint16_t to_fp16(float f) {
+  return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
+}
+__device__ __forceinline__ float from_bf16(uint32_t h) { return bits_f32(h << 16); }
+__device__ __forceinline__ float from_fp16(uint32_t h) {
+  return float(__builtin_bit_cast(_Float16, uint16_t(h)));
+}
+__device__ __forceinline__ uint16_t to_half(float f, int type) {
+  return type == I8CONV_BF16 ? to_bf16(f) : to_fp16(f);
+}
+__device__ __forceinline__ float from_half(uint32_t h, int type) {
+  return type == I8CONV_BF16 ? from_bf16(h) : from_fp16(h);
+}
+
+// One value of a row in memory.
+__device__ __forceinline__ float load_value(const void *p, int64_t i, int type) {
+  if (type == I8CONV_FP32) return static_cast<const float *>(p)[i];
+  return from_half(static_cast<const uint16_t *>(p)[i], type);
+}
+__device__ __forceinline__ void store_value(void *p, int64_t i, int type, float v) {
+  if (type == I8CONV_FP32)
+    static_cast<float *>(p)[i] = v;
+  else
+    static_cast<uint16_t *>(p)[i] = to_half(v, type);
+}
+// Four consecutive values, aligned to their size.
+__device__ __forceinline__ v4f load_values4(const void *p, int64_t i, int type) {
+  if (type == I8CONV_FP32) return *reinterpret_cast<const v4f *>(static_cast<const float *>(p) + i);
+  const v2u h = *reinterpret_cast<const v2u *>(static_cast<const uint16_t *>(p) + i);
+  return v4f{from_half(h[0] & 0xffffu, type), from_half(h[0] >> 16, type),
+             from_half(h[1] & 0xffffu, type), from_half(h[1] >> 16, type)};
+}
+__device__ __forceinline__ void store_values4(void *p, int64_t i, int type, v4f v) {
+  if (type == I8CONV_FP32) {
+    *reinterpret_cast<v4f *>(static_cast<float *>(p) + i) = v;
+    return;
+  }
+  const v2u h = {uint32_t(to_half(v[0], type)) | uint32_t(to_half(v[1], type)) << 16,
+                 uint32_t(to_half(v[2], type)) | uint32_t(to_half(v[3], type)) << 16};
+  *reinterpret_cast<v2u *>(static_cast<uint16_t *>(p) + i) = h;
+}
+
+// The activation of N values (a wave-uniform kind, chosen once for all of
+// them).  relu keeps NaN; the exponentials of large negative values overflow
+// to infinity and the quotients to -0, their limit.
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int kind) {
+  switch (kind) {
+    case I8CONV_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+      break;
+    case I8CONV_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678f));
+      break;
+    case I8CONV_ACT_GELU_TANH:
+      // 0.5 (1 + tanh(z)) = 1 / (1 + exp(-2 z))
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float z = v[i] * (1.5957691216f + 0.0713548162726f * v[i] * v[i]);
+        v[i] = v[i] / (1.0f + __expf(-z));
+      }
+      break;
+    case I8CONV_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = v[i] / (1.0f + __expf(-v[i]));
+      break;
+    default:
+      break;
+  }
+}
+
+#endif  // __HIPCC__
+
+}  // namespace i8conv
