@@ -216,12 +216,17 @@ int launch_transpose(const void *src, void *dst, int64_t batch, int rows, int co
                      void *stream);
 int launch_pack_vect(const int8_t *src, int8_t *dst, int n, int h, int w, int c, int vect,
                      bool unpack, void *stream);
-// kernel_quantize.hip, kernel_linear.hip, kernel_experts.hip: the int8 linear
+// kernel_quantize.hip, kernel_linear*.hip, kernel_experts.hip: the int8 linear
 // layers' launchers, on checked arguments (linear_capi.hip).
 struct LinearArgs;
 int launch_quantize(const void *x, int type, int64_t ldx, int rows, int k, int8_t *codes,
                     float *scales, void *stream);
 int launch_linear_tiles(const LinearArgs &a, bool gated, void *stream);
+// kernel_linear_rows.hip: layers of few rows.  fused: a.x holds 16-byte
+// aligned values of a.x_type, a row's stride a multiple of 16 bytes, which the
+// kernel quantizes itself, fused_rows(k) > 0 at a time; else codes.
+int fused_rows(int k);
+int launch_linear_rows(const LinearArgs &a, bool gated, bool fused, void *stream);
 int launch_route(const int32_t *ids, int tokens, int choices, int experts, int32_t *offsets,
                  int32_t *sources, int32_t *places, void *stream);
 int launch_combine(const void *x, int in_type, const int32_t *places, const float *weights,

@@ -117,7 +117,8 @@ __global__ __launch_bounds__(64 * WM * WN, kOcc) void linear_kernel(LinearArgs a
     const bool gather = kExperts && a.sources != nullptr;
     const int8_t *const wbase = a.w + int64_t(expert) * a.wide * a.k;
     const v4u wd = make_desc(wbase, uint32_t(a.wide) * uint32_t(a.k));
-    const int8_t *const xbase = gather ? a.x : a.x + int64_t(row0) * a.ldx;
+    const int8_t *const xbase =
+        static_cast<const int8_t *>(a.x) + (gather ? 0 : int64_t(row0) * a.ldx);
     const v4u xd = make_desc(xbase, gather ? uint32_t(int64_t(a.x_rows - 1) * a.ldx + a.k)
                                            : uint32_t((rows - 1) * uint32_t(a.ldx) + a.k));
     uint32_t aoff[CPA], boff[CPB];

@@ -2,6 +2,7 @@
 // which kernels a launch runs.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <string>
 
 #include "i8conv_internal.hpp"
@@ -80,6 +81,23 @@ int check_tensors(const i8conv_linear_shape &s, const void *input, const float *
   return I8CONV_OK;
 }
 
+// Which kernel runs a layer.
+struct RowsPlan {
+  bool few;    // kernel_linear_rows.hip instead of the tiles
+  bool fused;  // ... which quantizes the rows itself
+};
+RowsPlan plan_rows(const i8conv_linear_shape &s, const void *input) {
+  RowsPlan p{};
+  const int rows = s.experts ? s.routed : s.rows;
+  const int64_t ld = s.input_stride ? s.input_stride : s.inputs;
+  p.few = s.experts ? rows <= 4 * s.experts : rows <= 64;
+  p.fused = p.few && s.input_type != I8CONV_INT8 && aligned(input, 16) &&
+            ld * type_size(s.input_type) % 16 == 0 &&
+            (s.experts ? std::min(rows, s.rows) : rows) <= 16 && fused_rows(s.inputs) > 0 &&
+            (s.experts ? rows <= 2 * s.experts : rows <= fused_rows(s.inputs));
+  return p;
+}
+
 int run(const i8conv_linear_shape &s, const void *input, const float *input_scale,
         const int8_t *weight, const float *weight_scale, const float *bias, const void *residual,
         const int32_t *offsets, const int32_t *sources, void *output, void *workspace,
@@ -106,8 +124,10 @@ int run(const i8conv_linear_shape &s, const void *input, const float *input_scal
   a.out_type = s.output_type;
   a.vec = linear_vec_ok(output, a.ldy, a.n, size) &&
           (!residual || linear_vec_ok(residual, a.ldr, a.n, size));
-  if (s.input_type == I8CONV_INT8) {
-    a.x = static_cast<const int8_t *>(input);
+  const RowsPlan plan = plan_rows(s, input);
+  a.x_type = s.input_type;
+  if (plan.fused || s.input_type == I8CONV_INT8) {
+    a.x = input;
     a.xs = input_scale;
   } else {
     int8_t *const codes = static_cast<int8_t *>(workspace);
@@ -118,6 +138,7 @@ int run(const i8conv_linear_shape &s, const void *input, const float *input_scal
     a.xs = scales;
     a.ldx = s.inputs;
   }
+  if (plan.few) return launch_linear_rows(a, s.gated != 0, plan.fused, stream);
   return launch_linear_tiles(a, s.gated != 0, stream);
 }
 

@@ -13,8 +13,8 @@ namespace i8conv {
 
 // Arguments of a linear layer's product, dense or by expert.
 struct LinearArgs {
-  const int8_t *x;      // codes [x_rows][ldx]
-  const float *xs;      // [x_rows]
+  const void *x;        // [x_rows][ldx]: codes, or values of x_type
+  const float *xs;      // [x_rows], of codes
   const int8_t *w;      // [experts or 1][wide][k]
   const float *ws;      // [experts or 1][wide]
   const float *bias;    // [experts or 1][wide] or null
@@ -26,7 +26,7 @@ struct LinearArgs {
   int x_rows, rows;        // rows of x; rows of y (by expert: their upper bound)
   int k, n, wide;          // wide = n, or 2 n where gated
   int experts;             // 0: dense
-  int activation, out_type;
+  int activation, out_type, x_type;
   bool vec;  // four consecutive outputs may move at once (see linear_vec_ok)
 };
 
