@@ -221,7 +221,21 @@ int launch_pack_vect(const int8_t *src, int8_t *dst, int n, int h, int w, int c,
 struct LinearArgs;
 int launch_quantize(const void *x, int type, int64_t ldx, int rows, int k, int8_t *codes,
                     float *scales, void *stream);
-int launch_linear_tiles(const LinearArgs &a, bool gated, void *stream);
+// The tiles of kernel_linear.hip (rows x weight rows); Deep and Pair: small
+// grids, with four stage buffers and with two groups of waves to a tile.
+enum LinearTile {
+  kTile256x256,
+  kTile128x256,
+  kTile128x128,
+  kTile128x64,
+  kTile128x64Pair,  // gated only
+  kTile64x64,       // these not gated
+  kTile64x64Deep,
+  kTile64x64Pair
+};
+int launch_linear_tiles(const LinearArgs &a, bool gated, int tile, void *stream);
+// linear_policy.cpp: the tile for `rows` rows (of `experts` experts, 0: dense).
+int plan_linear_tile(int64_t rows, int64_t experts, int64_t n, int64_t k, bool gated);
 // kernel_linear_rows.hip: layers of few rows.  fused: a.x holds 16-byte
 // aligned values of a.x_type, a row's stride a multiple of 16 bytes, which the
 // kernel quantizes itself, fused_rows(k) > 0 at a time; else codes.

@@ -127,9 +127,9 @@ int launch_route(const int32_t *ids, int tokens, int choices, int experts, int32
 int launch_combine(const void *x, int in_type, const int32_t *places, const float *weights,
                    const void *residual, void *y, int out_type, int tokens, int choices, int n,
                    void *stream) {
-  const bool vec = linear_vec_ok(x, n, n, type_size(in_type)) &&
-                   linear_vec_ok(y, n, n, type_size(out_type)) &&
-                   (!residual || linear_vec_ok(residual, n, n, type_size(out_type)));
+  const bool vec = linear_vec_ok(x, n, n, type_size(in_type), 4) &&
+                   linear_vec_ok(y, n, n, type_size(out_type), 4) &&
+                   (!residual || linear_vec_ok(residual, n, n, type_size(out_type), 4));
   const unsigned parts = unsigned((n + 4 * kThreads - 1) / (4 * kThreads));
   I8_LAUNCH(combine_kernel, dim3(unsigned(tokens), parts), dim3(kThreads), 0,
             static_cast<hipStream_t>(stream), x, places, weights, residual, y, choices, n,

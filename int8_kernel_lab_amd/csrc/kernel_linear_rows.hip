@@ -280,7 +280,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void linear_rows_kernel(LinearArgs
           for (int e = 0; e < 4; ++e) v[e] *= u[e];
         }
         const int64_t row = row0 + r;
-        if (a.vec) {
+        if (a.vec4) {
           v4f o = {v[0], v[1], v[2], v[3]};
           if (a.residual) o += load_values4(a.residual, row * a.ldr + ch, a.out_type);
           store_values4(a.y, row * a.ldy + ch, a.out_type, o);

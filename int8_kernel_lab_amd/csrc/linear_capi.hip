@@ -122,8 +122,12 @@ int run(const i8conv_linear_shape &s, const void *input, const float *input_scal
   a.experts = s.experts;
   a.activation = s.activation;
   a.out_type = s.output_type;
-  a.vec = linear_vec_ok(output, a.ldy, a.n, size) &&
-          (!residual || linear_vec_ok(residual, a.ldr, a.n, size));
+  const auto vec_ok = [&](int count) {
+    return linear_vec_ok(output, a.ldy, a.n, size, count) &&
+           (!residual || linear_vec_ok(residual, a.ldr, a.n, size, count));
+  };
+  a.vec4 = vec_ok(4);
+  a.vec2 = vec_ok(2) && a.ldy < kVec2MaxStride && (!residual || a.ldr < kVec2MaxStride);
   const RowsPlan plan = plan_rows(s, input);
   a.x_type = s.input_type;
   if (plan.fused || s.input_type == I8CONV_INT8) {
@@ -139,7 +143,8 @@ int run(const i8conv_linear_shape &s, const void *input, const float *input_scal
     a.ldx = s.inputs;
   }
   if (plan.few) return launch_linear_rows(a, s.gated != 0, plan.fused, stream);
-  return launch_linear_tiles(a, s.gated != 0, stream);
+  const int tile = plan_linear_tile(a.rows, a.experts, a.n, a.k, s.gated != 0);
+  return launch_linear_tiles(a, s.gated != 0, tile, stream);
 }
 
 int check_route(const i8conv_route_shape *s) {

@@ -27,14 +27,17 @@ struct LinearArgs {
   int k, n, wide;          // wide = n, or 2 n where gated
   int experts;             // 0: dense
   int activation, out_type, x_type;
-  bool vec;  // four consecutive outputs may move at once (see linear_vec_ok)
+  bool vec4, vec2;  // outputs may move four or two at once (linear_vec_ok)
 };
 
-// Whether rows of n values of `size` bytes at base + row * ld may be moved four
-// at a time.
-inline bool linear_vec_ok(const void *base, int64_t ld, int n, int size) {
-  return n % 4 == 0 && ld % 4 == 0 && (reinterpret_cast<uintptr_t>(base) & (4 * size - 1)) == 0;
+// Whether rows of n values of `size` bytes at base + row * ld may be moved
+// `count` at a time.
+inline bool linear_vec_ok(const void *base, int64_t ld, int n, int size, int count) {
+  return n % count == 0 && ld % count == 0 &&
+         (reinterpret_cast<uintptr_t>(base) & uintptr_t(count * size - 1)) == 0;
 }
+// The two-wide form addresses a tile's rows with 32-bit offsets.
+constexpr int64_t kVec2MaxStride = int64_t(1) << 20;
 
 I8_HD inline int type_size(int type) {
   return type == I8CONV_INT8 ? 1 : type == I8CONV_FP32 ? 4 : 2;
@@ -51,6 +54,8 @@ __device__ __forceinline__ uint32_t f32_bits(float f) { return __builtin_bit_cas
 __device__ __forceinline__ uint16_t to_bf16(float f) {
   return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f));  // to nearest even
 }
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint16_t to_fp16(float f) {
   return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
 }
@@ -63,6 +68,13 @@ __device__ __forceinline__ uint16_t to_half(float f, int type) {
 }
 __device__ __forceinline__ float from_half(uint32_t h, int type) {
   return type == I8CONV_BF16 ? from_bf16(h) : from_fp16(h);
+}
+
+// Two values in a dword, the first in its low half.
+__device__ __forceinline__ uint32_t to_halves(float lo, float hi, int type) {
+  if (type == I8CONV_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{lo, hi}, v2bf));
+  return uint32_t(to_fp16(lo)) | uint32_t(to_fp16(hi)) << 16;
 }
 
 // One value of a row in memory.
@@ -93,34 +105,27 @@ __device__ __forceinline__ void store_values4(void *p, int64_t i, int type, v4f 
   *reinterpret_cast<v2u *>(static_cast<uint16_t *>(p) + i) = h;
 }
 
-// The activation of N values (a wave-uniform kind, chosen once for all of
-// them).  relu keeps NaN; the exponentials of large negative values overflow
-// to infinity and the quotients to -0, their limit.
+// The activation of N values, of a wave-uniform kind.  relu keeps NaN.
+// gelu_tanh and silu are both v times the logistic function of a polynomial:
+// 0.5 (1 + tanh(z / 2)) = 1 / (1 + exp(-z)); their exponentials overflow to
+// infinity for large negative values and the product is then -0, the limit.
 template <int N>
 __device__ __forceinline__ void activate(float (&v)[N], int kind) {
-  switch (kind) {
-    case I8CONV_ACT_RELU:
+  if (kind <= I8CONV_ACT_RELU) {
+    const float floor = kind == I8CONV_ACT_RELU ? 0.0f : -__builtin_inff();
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
-      break;
-    case I8CONV_ACT_GELU:
+    for (int i = 0; i < N; ++i) v[i] = v[i] < floor ? floor : v[i];
+  } else if (kind == I8CONV_ACT_GELU) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678f));
-      break;
-    case I8CONV_ACT_GELU_TANH:
-      // 0.5 (1 + tanh(z)) = 1 / (1 + exp(-2 z))
+    for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678f));
+  } else {
+    const float c1 = kind == I8CONV_ACT_SILU ? 1.0f : 1.5957691216f;
+    const float c3 = kind == I8CONV_ACT_SILU ? 0.0f : 0.0713548162726f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float z = v[i] * (1.5957691216f + 0.0713548162726f * v[i] * v[i]);
-        v[i] = v[i] / (1.0f + __expf(-z));
-      }
-      break;
-    case I8CONV_ACT_SILU:
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = v[i] / (1.0f + __expf(-v[i]));
-      break;
-    default:
-      break;
+    for (int i = 0; i < N; ++i) {
+      const float z = v[i] * fmaf(c3 * v[i], v[i], c1);
+      v[i] *= __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+    }
   }
 }
 

@@ -1,0 +1,61 @@
+// Which kernel runs an int8 linear layer: the policy of the linear layers, kept
+// outside the kernels like that of the convolutions (policy.cpp).
+#include <algorithm>
+
+#include "i8conv_internal.hpp"
+#include "linear_common.hpp"
+
+namespace i8conv {
+namespace {
+
+// A tile of kernel_linear.hip and what it takes, in us: a 128-byte k-stage with
+// one workgroup on a compute unit and few of them busy (`alone`), with all of
+// them full (`full`), and what a tile costs besides its stages.  Read off
+// sweeps of 80 to 4096 rows over 1024 to 12288 columns, 1024 to 8192 deep, on
+// all tiles.
+struct TileCost {
+  int tile, bm, bn, per_unit, kg;
+  bool plain, gated;
+  double alone, full, besides;
+};
+const TileCost kTiles[] = {
+    {kTile256x256, 256, 256, 1, 1, true, true, 1.25, 1.80, 5.0},
+    {kTile128x256, 128, 256, 1, 1, true, true, 0.76, 1.10, 4.0},
+    {kTile128x128, 128, 128, 2, 1, true, true, 0.66, 1.18, 3.0},
+    {kTile128x64, 128, 64, 3, 1, true, true, 0.60, 1.05, 2.5},
+    {kTile64x64, 64, 64, 4, 1, true, false, 0.50, 0.90, 2.0},
+    {kTile64x64Deep, 64, 64, 2, 1, true, false, 0.28, 0.45, 2.0},
+    {kTile64x64Pair, 64, 64, 1, 2, true, false, 0.42, 0.50, 2.5},
+    {kTile128x64Pair, 128, 64, 1, 2, false, true, 0.60, 0.76, 2.5},
+};
+
+double cost(const TileCost &t, int64_t row_tiles, int64_t wide, int64_t k) {
+  const int64_t tiles = row_tiles * ((wide + t.bn - 1) / t.bn);
+  const int64_t slots = 256 * t.per_unit, rounds = tiles / slots, rest = tiles % slots;
+  const double stages = double((k + 128 * t.kg - 1) / (128 * t.kg));
+  double us = double(rounds) * (stages * t.full + t.besides);
+  if (rest) {
+    // the last round: how full its compute units are
+    const double fill = double(rest) / double(slots);
+    us += stages * (t.alone + (t.full - t.alone) * fill) + t.besides;
+  }
+  return us;
+}
+
+}  // namespace
+
+int plan_linear_tile(int64_t rows, int64_t experts, int64_t n, int64_t k, bool gated) {
+  int best = kTile128x128;
+  double least = 1e300;
+  for (const TileCost &t : kTiles) {
+    if (gated ? !t.gated : !t.plain) continue;
+    int64_t row_tiles = (rows + t.bm - 1) / t.bm;
+    // by expert: each group ends in a part of a tile, in the mean half of one
+    if (experts) row_tiles = rows / t.bm + (std::min(experts, rows) + 1) / 2;
+    const double us = cost(t, row_tiles, gated ? 2 * n : n, k);
+    if (us < least) least = us, best = t.tile;
+  }
+  return best;
+}
+
+}  // namespace i8conv
