@@ -238,11 +238,12 @@ int launch_linear_tiles(const LinearArgs &a, bool gated, int tile, void *stream)
 int plan_linear_tile(int64_t rows, int64_t experts, int64_t n, int64_t k, bool gated);
 // kernel_linear_rows.hip: layers of few rows.  fused: a.x holds 16-byte
 // aligned values of a.x_type, a row's stride a multiple of 16 bytes, which the
-// kernel quantizes itself, fused_rows(k) > 0 at a time; else codes.
-int fused_rows(int k);
+// kernel quantizes itself, fused_rows(k, value bytes) > 0 at a time; else codes.
+int fused_rows(int k, int size);
 int launch_linear_rows(const LinearArgs &a, bool gated, bool fused, void *stream);
+size_t route_workspace(int64_t ids, int experts);
 int launch_route(const int32_t *ids, int tokens, int choices, int experts, int32_t *offsets,
-                 int32_t *sources, int32_t *places, void *stream);
+                 int32_t *sources, int32_t *places, void *workspace, void *stream);
 int launch_combine(const void *x, int in_type, const int32_t *places, const float *weights,
                    const void *residual, void *y, int out_type, int tokens, int choices, int n,
                    void *stream);

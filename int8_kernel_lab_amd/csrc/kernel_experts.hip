@@ -68,42 +68,169 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(const int32_t *ids
     for (int i = total + int(threadIdx.x); i < count; i += kRouteThreads) sources[i] = -1;
 }
 
-// A workgroup per token and 1024 outputs, four outputs a thread.
+// Long lists, two launches over parts of kPartIds ids.  First the experts'
+// counts of each part.  Then a workgroup per part has the part's first row of
+// every expert from the counts of the parts before, and the rows of its waves'
+// segments from counts of its own; a wave ranks 64 ids at a time by the lanes
+// with the same id, one ballot per bit of an id.
+constexpr int kPartIds = 4096, kWaveIds = kPartIds / kRouteWaves;
+__global__ __launch_bounds__(kRouteThreads) void route_count_kernel(const int32_t *ids, int count,
+                                                                   int experts, int32_t *counts) {
+  extern __shared__ int sum[];
+  for (int e = threadIdx.x; e < experts; e += kRouteThreads) sum[e] = 0;
+  __syncthreads();
+  const int begin = int(blockIdx.x) * kPartIds;
+#pragma unroll
+  for (int u = 0; u < kPartIds / kRouteThreads; ++u) {
+    const int i = begin + u * kRouteThreads + int(threadIdx.x);
+    const int id = i < count ? ids[i] : -1;
+    if (id >= 0 && id < experts) atomicAdd(&sum[id], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += kRouteThreads)
+    counts[int64_t(blockIdx.x) * experts + e] = sum[e];
+}
+
+__global__ __launch_bounds__(kRouteThreads) void route_place_kernel(
+    const int32_t *ids, int count, int choices, int experts, int id_bits, const int32_t *counts,
+    int32_t *offsets, int32_t *sources, int32_t *places) {
+  extern __shared__ int next[];  // [waves][experts], then the waves' totals
+  int *const totals = next + kRouteWaves * experts;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int part = blockIdx.x, parts = gridDim.x;
+  const int begin = part * kPartIds + wave * kWaveIds;
+  int id[kWaveIds / 64];
+#pragma unroll
+  for (int u = 0; u < kWaveIds / 64; ++u) {
+    const int i = begin + u * 64 + lane;
+    id[u] = i < count ? ids[i] : -1;
+    if (id[u] >= experts) id[u] = -1;
+  }
+  for (int e = threadIdx.x; e < kRouteWaves * experts; e += kRouteThreads) next[e] = 0;
+  __syncthreads();
+  // (whole numbers: the order of the additions does not show)
+#pragma unroll
+  for (int u = 0; u < kWaveIds / 64; ++u)
+    if (id[u] >= 0) atomicAdd(&next[wave * experts + id[u]], 1);
+  // expert threadIdx.x (experts <= kRouteThreads): its rows before this part and in all
+  const int e = threadIdx.x;
+  int before = 0, all = 0;
+  if (e < experts)
+    for (int p = 0; p < parts; ++p) {
+      const int c = counts[int64_t(p) * experts + e];
+      before += p < part ? c : 0;
+      all += c;
+    }
+  int sum = all;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int up = __shfl_up(sum, d);
+    sum += lane >= d ? up : 0;
+  }
+  if (lane == 63) totals[wave] = sum;
+  __syncthreads();
+  int base = sum - all, total = 0;
+  for (int w = 0; w < kRouteWaves; ++w) {
+    if (w < wave) base += totals[w];
+    total += totals[w];
+  }
+  if (e < experts) {
+    if (part == 0) offsets[e] = base;
+    int row = base + before;
+    for (int w = 0; w < kRouteWaves; ++w) {
+      const int c = next[w * experts + e];
+      next[w * experts + e] = row;
+      row += c;
+    }
+  }
+  if (part == 0 && e == 0) offsets[experts] = total;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kWaveIds / 64; ++u) {
+    const int i = begin + u * 64 + lane;
+    const bool live = id[u] >= 0;
+    uint64_t same = __ballot(live);
+    for (int b = 0; b < id_bits; ++b) {
+      const uint64_t ones = __ballot(id[u] >> b & 1);
+      same &= id[u] >> b & 1 ? ones : ~ones;
+    }
+    const int rank = __popcll(same & ((uint64_t(1) << lane) - 1));
+    int row = -1;
+    if (live) {
+      // every lane reads its expert's row before the first of its equals moves it on
+      row = next[wave * experts + id[u]] + rank;
+      if (rank == 0) next[wave * experts + id[u]] = row + __popcll(same);
+    }
+    if (i < count) {
+      places[i] = row;
+      if (live) sources[row] = i / choices;
+    }
+  }
+  // sources past the last row, shared among the parts
+  for (int64_t i = total + int64_t(part) * kRouteThreads + threadIdx.x; i < count;
+       i += int64_t(parts) * kRouteThreads)
+    sources[i] = -1;
+}
+
+// A token's rows are read four at a time, eight values of 16 bits or four of 32
+// per thread (kVec; else single ones).
+template <bool kVec, int V>
 __global__ __launch_bounds__(kThreads) void combine_kernel(const void *x, const int32_t *places,
                                                            const float *weights,
                                                            const void *residual, void *y,
-                                                           int choices, int n, int rows,
-                                                           int in_type, int out_type, int vec) {
-  const int64_t t = blockIdx.x;
-  const int c0 = (int(blockIdx.y) * kThreads + int(threadIdx.x)) * 4;
+                                                           int64_t tokens, int choices, int n,
+                                                           int rows, int in_type, int out_type) {
+  const int c0 = (int(blockIdx.y) * kThreads + int(threadIdx.x)) * V;
   if (c0 >= n) return;
-  const int live = min(4, n - c0);
-  v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int c = 0; c < choices; ++c) {
-    const int row = places[t * choices + c];
-    if (row < 0 || row >= rows) continue;
-    const float wt = weights[t * choices + c];
-    const int64_t at = int64_t(row) * n + c0;
-    if (vec) {
-      const v4f v = load_values4(x, at, in_type);
+  const int live = min(V, n - c0);
+  for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x) {
+    float sum[V];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] = fmaf(wt, v[e], sum[e]);
+    for (int e = 0; e < V; ++e) sum[e] = 0.0f;
+    for (int c = 0; c < choices; c += 4) {
+      float v[4][V];
+      bool ok[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int row = c + u < choices ? places[t * choices + c + u] : -1;
+        ok[u] = row >= 0 && row < rows;
+        if (!ok[u]) continue;
+        const int64_t at = int64_t(row) * n + c0;
+        if constexpr (kVec) {
+#pragma unroll
+          for (int e = 0; e < V; e += 4) {
+            const v4f q = load_values4(x, at + e, in_type);
+#pragma unroll
+            for (int f = 0; f < 4; ++f) v[u][e + f] = q[f];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[u][e] = e < live ? load_value(x, at + e, in_type) : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (!ok[u]) continue;  // its row and its weight may hold anything
+        const float w = weights[t * choices + c + u];
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] = fmaf(w, v[u][e], sum[e]);
+      }
+    }
+    const int64_t at = t * n + c0;
+    if constexpr (kVec) {
+#pragma unroll
+      for (int e = 0; e < V; e += 4) {
+        v4f q = {sum[e], sum[e + 1], sum[e + 2], sum[e + 3]};
+        if (residual) q += load_values4(residual, at + e, out_type);
+        store_values4(y, at + e, out_type, q);
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < live) sum[e] = fmaf(wt, load_value(x, at + e, in_type), sum[e]);
+      for (int e = 0; e < V; ++e)
+        if (e < live)
+          store_value(y, at + e, out_type,
+                      residual ? sum[e] + load_value(residual, at + e, out_type) : sum[e]);
     }
-  }
-  const int64_t at = t * n + c0;
-  if (vec) {
-    if (residual) sum += load_values4(residual, at, out_type);
-    store_values4(y, at, out_type, sum);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < live)
-        store_value(y, at + e, out_type,
-                    residual ? sum[e] + load_value(residual, at + e, out_type) : sum[e]);
   }
 }
 
@@ -116,24 +243,59 @@ int done(const char *what) {
 
 }  // namespace
 
+// Lists from this many ids on take the two launches: 131072 ids of 128 experts
+// 64 us with a workgroup per expert, which reads all of them twice.
+constexpr int kRouteLong = 8192;
+bool route_long(int64_t ids, int experts) { return ids >= kRouteLong && experts <= kRouteThreads; }
+
+size_t route_workspace(int64_t ids, int experts) {
+  return route_long(ids, experts) ? size_t((ids + kPartIds - 1) / kPartIds) * size_t(experts) * 4 : 0;
+}
+
 int launch_route(const int32_t *ids, int tokens, int choices, int experts, int32_t *offsets,
-                 int32_t *sources, int32_t *places, void *stream) {
-  I8_LAUNCH(route_kernel, dim3(unsigned(experts)), dim3(kRouteThreads), 0,
-            static_cast<hipStream_t>(stream), ids, tokens * choices, choices, experts, offsets,
-            sources, places);
+                 int32_t *sources, int32_t *places, void *workspace, void *stream) {
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int count = tokens * choices;
+  if (!route_long(count, experts)) {
+    I8_LAUNCH(route_kernel, dim3(unsigned(experts)), dim3(kRouteThreads), 0, s, ids, count, choices,
+              experts, offsets, sources, places);
+    return done("route launch");
+  }
+  int32_t *const counts = static_cast<int32_t *>(workspace);
+  const unsigned parts = unsigned((int64_t(count) + kPartIds - 1) / kPartIds);
+  int id_bits = 0;
+  while ((1 << id_bits) < experts) ++id_bits;
+  I8_LAUNCH(route_count_kernel, dim3(parts), dim3(kRouteThreads), size_t(experts) * 4, s, ids, count,
+            experts, counts);
+  const size_t lds = size_t(kRouteWaves) * experts * 4 + kRouteWaves * 4;
+  static LdsLimit limit;
+  if (const int rc = limit.raise(route_place_kernel, lds); rc != I8CONV_OK) return rc;
+  I8_LAUNCH(route_place_kernel, dim3(parts), dim3(kRouteThreads), lds, s, ids, count, choices, experts,
+            id_bits, counts, offsets, sources, places);
   return done("route launch");
 }
 
 int launch_combine(const void *x, int in_type, const int32_t *places, const float *weights,
                    const void *residual, void *y, int out_type, int tokens, int choices, int n,
                    void *stream) {
-  const bool vec = linear_vec_ok(x, n, n, type_size(in_type), 4) &&
-                   linear_vec_ok(y, n, n, type_size(out_type), 4) &&
-                   (!residual || linear_vec_ok(residual, n, n, type_size(out_type), 4));
-  const unsigned parts = unsigned((n + 4 * kThreads - 1) / (4 * kThreads));
-  I8_LAUNCH(combine_kernel, dim3(unsigned(tokens), parts), dim3(kThreads), 0,
-            static_cast<hipStream_t>(stream), x, places, weights, residual, y, choices, n,
-            tokens * choices, in_type, out_type, int(vec));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const auto vec_ok = [&](int count) {
+    return linear_vec_ok(x, n, n, type_size(in_type), 4) && n % count == 0 &&
+           linear_vec_ok(y, n, n, type_size(out_type), 4) &&
+           (!residual || linear_vec_ok(residual, n, n, type_size(out_type), 4));
+  };
+  const unsigned blocks = unsigned(std::min(tokens, 1 << 20));
+  const auto launch = [&](auto kern, int v) {
+    const unsigned parts = unsigned((int64_t(n) + v * kThreads - 1) / (v * kThreads));
+    I8_LAUNCH(kern, dim3(blocks, parts), dim3(kThreads), 0, s, x, places, weights, residual, y,
+              int64_t(tokens), choices, n, tokens * choices, in_type, out_type);
+  };
+  if (vec_ok(8) && type_size(in_type) == 2)
+    launch(combine_kernel<true, 8>, 8);
+  else if (vec_ok(4))
+    launch(combine_kernel<true, 4>, 4);
+  else
+    launch(combine_kernel<false, 4>, 4);
   return done("combine launch");
 }
 

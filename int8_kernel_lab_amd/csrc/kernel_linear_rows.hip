@@ -8,7 +8,7 @@
 // at a time and the next one before the first is used, and ends with four
 // consecutive channels of row l % 16.
 //
-// The rows come as codes, from memory like the weights (kDirect), or as floating-point
+// The rows come as codes, from memory like the weights, or as floating-point
 // values that the workgroup quantizes itself into LDS (kFused), while its first
 // weights are on the way: every workgroup does that work again, but a launch
 // and the codes' way through memory are saved.
@@ -29,9 +29,10 @@ namespace i8conv {
 namespace {
 
 constexpr int kRowsWaves = 8, kRowsThreads = 64 * kRowsWaves;
-constexpr int kFusedChunks = 4;  // 8-value pieces of x a thread holds
-constexpr int kFusedLds = 256;   // bytes of their largest values and the rows' scales
-static_assert(kFusedChunks * (kRowsWaves + 1) * 4 <= kFusedLds, "fits");
+// 8-value pieces of x a thread holds: 16 registers of 16-bit or 32-bit values.
+constexpr int fused_chunks(int size) { return size == 4 ? 2 : 4; }
+constexpr int kFusedLds = 256;  // bytes of their largest values and the rows' scales
+static_assert(fused_chunks(2) * (kRowsWaves + 1) * 4 <= kFusedLds, "fits");
 
 // Bytes between rows of codes in LDS: 16-byte units in a step of 2 x odd, so
 // that a fragment read (16 rows, two chunks per 32 lanes) has no bank conflicts.
@@ -65,17 +66,23 @@ __device__ __forceinline__ bool find_group(const int32_t *offsets, int experts, 
   return false;
 }
 
-// MF: fragments of 16 rows taken together; U: k-steps of 64 bytes per batch.
-template <bool kGated, bool kExperts, bool kFused, int MF, int U>
-__global__ __launch_bounds__(kRowsThreads, 2) void linear_rows_kernel(LinearArgs a) {
-  constexpr int F = kGated ? 2 : 1;
+// C: times 16 channels (of each half) per workgroup; kX: bytes of a value to
+// quantize, 0 for codes; MF: fragments of 16 rows taken
+// together; U: k-steps of 64 bytes per batch.  A workgroup's life is mostly
+// waiting (group, sources, rows, weights, one after the other), so kOcc waves
+// per SIMD keep several workgroups on a compute unit.
+template <bool kGated, bool kExperts, int kX, int C, int MF, int U, int kOcc>
+__global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearArgs a) {
+  constexpr int F = kGated ? 2 * C : C;
+  constexpr bool kFused = kX != 0;
+  constexpr int kChunks = fused_chunks(kX);
   // LDS: the waves' sums; kFused: the pieces' largest values, the rows' scales
   // and their codes [step_rows][pitch]
   extern __shared__ __attribute__((aligned(16))) int8_t smem[];
   v4i(*const sums)[F * MF][64] = reinterpret_cast<v4i(*)[F * MF][64]>(smem);
   int8_t *const extra = smem + sizeof(v4i) * kRowsWaves * F * MF * 64;
   uint32_t(*const tops)[kRowsWaves] = reinterpret_cast<uint32_t(*)[kRowsWaves]>(extra);
-  float *const row_scale = reinterpret_cast<float *>(extra + kFusedChunks * kRowsWaves * 4);
+  float *const row_scale = reinterpret_cast<float *>(extra + kChunks * kRowsWaves * 4);
   int8_t *const codes = extra + kFusedLds;
 
   const int lane = threadIdx.x & 63;
@@ -89,7 +96,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void linear_rows_kernel(LinearArgs
   }
   const bool gather = kExperts && a.sources != nullptr;
   const int q = lane & 15, kq = 16 * (lane >> 4);
-  const int c0 = int(blockIdx.x) * 16;
+  const int c0 = int(blockIdx.x) * 16 * C;
 
   // this wave's part of the reduction
   const int steps = (a.k + 63) / 64, per = (steps + kRowsWaves - 1) / kRowsWaves;
@@ -98,8 +105,10 @@ __global__ __launch_bounds__(kRowsThreads, 2) void linear_rows_kernel(LinearArgs
   const auto wr = make_rsrc(a.w + int64_t(group.expert) * a.wide * a.k, uint32_t(a.wide) * uint32_t(a.k));
   uint32_t woff[F];
 #pragma unroll
-  for (int f = 0; f < F; ++f)
-    woff[f] = c0 + q < a.n ? uint32_t(c0 + q + (f ? a.n : 0)) * uint32_t(a.k) + uint32_t(kq) : kOutOfRange;
+  for (int f = 0; f < F; ++f) {
+    const int ch = c0 + 16 * (f % C) + q;
+    woff[f] = ch < a.n ? uint32_t(ch + (f >= C ? a.n : 0)) * uint32_t(a.k) + uint32_t(kq) : kOutOfRange;
+  }
   auto load_w = [&](v4i (&wv)[U][F], int k) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -113,11 +122,11 @@ __global__ __launch_bounds__(kRowsThreads, 2) void linear_rows_kernel(LinearArgs
   const int pitch = fused_pitch(a.k);
   // rows of x per pass
   const int chunks = (a.k + 8 * kRowsThreads - 1) / (8 * kRowsThreads);
-  const int step_rows = kFused ? kFusedChunks / chunks : 16 * MF;
+  const int step_rows = kFused ? kChunks / chunks : 16 * MF;
   for (int row0 = group.begin; row0 < group.end; row0 += step_rows) {
     const int rows = min(step_rows, group.end - row0);
 
-    // kDirect: this lane's row of each fragment
+    // codes: this lane's row of each fragment
     uint32_t xoff[MF];
     const int8_t *const xbase =
         static_cast<const int8_t *>(a.x) + (gather || kFused ? 0 : int64_t(row0) * a.ldx);
@@ -143,63 +152,43 @@ __global__ __launch_bounds__(kRowsThreads, 2) void linear_rows_kernel(LinearArgs
 #pragma unroll
       for (int m = 0; m < MF; ++m) acc[f][m] = v4i{0, 0, 0, 0};
 
-    v4i wv[2][U][F], xv[2][U][MF];
-    auto load_x = [&](v4i (&dst)[U][MF], int k) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int m = 0; m < MF; ++m) {
-          const bool ok = k + 64 * u + kq < k1;
-          if constexpr (kFused)
-            dst[u][m] = ok ? *reinterpret_cast<const v4i *>(codes + min(q, rows - 1) * pitch + k + 64 * u + kq)
-                           : v4i{0, 0, 0, 0};
-          else
-            dst[u][m] = load16(xr, ok && xoff[m] != kOutOfRange ? xoff[m] + uint32_t(k + 64 * u)
-                                                               : kOutOfRange);
-        }
-    };
-    auto multiply = [&](const v4i (&w)[U][F], const v4i (&x)[U][MF]) {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int f = 0; f < F; ++f)
-#pragma unroll
-          for (int m = 0; m < MF; ++m) acc[f][m] = mfma16(w[u][f], x[u][m], acc[f][m]);
-    };
-
+    v4i wv[U][F];
     if constexpr (kFused) {
       // the values first, then the first weights: loads return in order
-      v4f v[kFusedChunks][2];
+      constexpr int kWords = kX == 4 ? 8 : 4;  // of a piece
+      uint32_t raw[kChunks][kWords];
       const int piece = int(threadIdx.x) * 8;
-      auto read = [&](auto type) {
+      {
         int r = 0, c = 0;  // piece i is piece c of row r
 #pragma unroll
-        for (int i = 0; i < kFusedChunks; ++i, ++c) {
+        for (int i = 0; i < kChunks; ++i, ++c) {
           if (c == chunks) c = 0, ++r;
           const int k = piece + c * 8 * kRowsThreads;
-          float t[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-          if (r < rows && k < a.k) {
-            int64_t src = row0 + r;
-            if (gather) src = a.sources[src];
-            if (uint64_t(src) < uint64_t(a.x_rows)) load8<decltype(type)::value, true>(a.x, src * a.ldx + k, t);
+          int64_t src = row0 + r;
+          bool ok = r < rows && k < a.k;
+          if (gather && ok) src = a.sources[src];
+          ok = ok && uint64_t(src) < uint64_t(a.x_rows);
+          const int8_t *const p = static_cast<const int8_t *>(a.x) + (src * a.ldx + k) * kX;
+#pragma unroll
+          for (int w = 0; w < kWords; w += 4) {
+            const v4u t = ok ? *reinterpret_cast<const v4u *>(p + 4 * w) : v4u{0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) raw[i][w + e] = t[e];
           }
-          v[i][0] = v4f{t[0], t[1], t[2], t[3]};
-          v[i][1] = v4f{t[4], t[5], t[6], t[7]};
         }
-      };
-      if (a.x_type == I8CONV_BF16)
-        read(std::integral_constant<int, I8CONV_BF16>{});
-      else if (a.x_type == I8CONV_FP16)
-        read(std::integral_constant<int, I8CONV_FP16>{});
-      else
-        read(std::integral_constant<int, I8CONV_FP32>{});
-      load_w(wv[0], k0);
+      }
+      load_w(wv, k0);
       auto piece_of = [&](int i, float (&t)[8]) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = v[i][e / 4][e % 4];
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (kX == 4)
+            t[e] = bits_f32(raw[i][e]);
+          else
+            t[e] = from_half(raw[i][e / 2] >> (16 * (e & 1)) & 0xffffu, a.x_type);
+        }
       };
 #pragma unroll
-      for (int i = 0; i < kFusedChunks; ++i) {
+      for (int i = 0; i < kChunks; ++i) {
         float t[8];
         piece_of(i, t);
         const uint32_t top = wave_max(top8(t));
@@ -208,7 +197,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void linear_rows_kernel(LinearArgs
       __syncthreads();
       int r = 0, c = 0;
 #pragma unroll
-      for (int i = 0; i < kFusedChunks; ++i, ++c) {
+      for (int i = 0; i < kChunks; ++i, ++c) {
         if (c == chunks) c = 0, ++r;
         const int k = piece + c * 8 * kRowsThreads;
         if (r >= rows) break;
@@ -223,23 +212,31 @@ __global__ __launch_bounds__(kRowsThreads, 2) void linear_rows_kernel(LinearArgs
         if (k < a.k) *reinterpret_cast<v2u *>(codes + r * pitch + k) = codes8(t, step);
       }
       __syncthreads();
-      load_x(xv[0], k0);
     } else {
-      load_w(wv[0], k0);
-      load_x(xv[0], k0);
+      load_w(wv, k0);
     }
-    for (int k = k0; k < k1; k += 128 * U) {
-      if (k + 64 * U < k1) {
-        load_w(wv[1], k + 64 * U);
-        load_x(xv[1], k + 64 * U);
-      }
-      multiply(wv[0], xv[0]);
-      if (k + 64 * U >= k1) break;
-      if (k + 128 * U < k1) {
-        load_w(wv[0], k + 128 * U);
-        load_x(xv[0], k + 128 * U);
-      }
-      multiply(wv[1], xv[1]);
+#pragma unroll 1
+    for (int k = k0; k < k1; k += 64 * U) {
+      if (k > k0) load_w(wv, k);
+      v4i xv[U][MF];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int m = 0; m < MF; ++m) {
+          const int kk = k + 64 * u;
+          const bool ok = kk + kq < k1;
+          if constexpr (kFused)
+            xv[u][m] = ok ? *reinterpret_cast<const v4i *>(codes + min(q, rows - 1) * pitch + kk + kq)
+                          : v4i{0, 0, 0, 0};
+          else
+            xv[u][m] = load16(xr, ok && xoff[m] != kOutOfRange ? xoff[m] + uint32_t(kk) : kOutOfRange);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+#pragma unroll
+          for (int m = 0; m < MF; ++m) acc[f][m] = mfma16(wv[u][f], xv[u][m], acc[f][m]);
     }
 
 #pragma unroll
@@ -247,14 +244,17 @@ __global__ __launch_bounds__(kRowsThreads, 2) void linear_rows_kernel(LinearArgs
 #pragma unroll
       for (int m = 0; m < MF; ++m) sums[wave][f * MF + m][lane] = acc[f][m];
     __syncthreads();
-    if (wave < MF) {
-      const int m = wave, r = 16 * m + q, ch = c0 + 4 * (lane >> 4);
-      v4i s[F];
+    // each wave finishes 16 channels of 16 rows
+    for (int part = wave; part < C * MF; part += kRowsWaves) {
+      const int m = part % MF, c = part / MF;
+      const int r = 16 * m + q, ch = c0 + 16 * c + 4 * (lane >> 4);
+      v4i s[kGated ? 2 : 1];
 #pragma unroll
-      for (int f = 0; f < F; ++f) {
-        s[f] = sums[0][f * MF + m][lane];
-#pragma unroll
-        for (int w = 1; w < kRowsWaves; ++w) s[f] += sums[w][f * MF + m][lane];
+      for (int h = 0; h < (kGated ? 2 : 1); ++h) {
+        const int f = (h * C + c) * MF + m;
+        s[h] = sums[0][f][lane];
+#pragma unroll 2  // (all of them at once take as many registers as the rest)
+        for (int w = 1; w < kRowsWaves; ++w) s[h] += sums[w][f][lane];
       }
       if (r < rows && ch < a.n) {
         float xs;
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void linear_rows_kernel(LinearArgs
           const bool ok = ch + e < a.n;
           v[e] = fmaf(float(s[0][e]) * xs, ok ? a.ws[p + e] : 0.0f, ok && a.bias ? a.bias[p + e] : 0.0f);
           if constexpr (kGated)
-            u[e] = fmaf(float(s[F - 1][e]) * xs, ok ? a.ws[p + a.n + e] : 0.0f,
+            u[e] = fmaf(float(s[kGated][e]) * xs, ok ? a.ws[p + a.n + e] : 0.0f,
                         ok && a.bias ? a.bias[p + a.n + e] : 0.0f);
         }
         activate(v, a.activation);
@@ -299,14 +299,14 @@ __global__ __launch_bounds__(kRowsThreads, 2) void linear_rows_kernel(LinearArgs
   }
 }
 
-template <bool kGated, bool kExperts, bool kFused, int MF, int U>
+template <bool kGated, bool kExperts, int kX, int C, int MF, int U, int kOcc>
 int launch_rows(const LinearArgs &a, hipStream_t s) {
-  auto kern = linear_rows_kernel<kGated, kExperts, kFused, MF, U>;
-  const size_t lds = size_t(kRowsWaves) * (kGated ? 2 : 1) * MF * 1024 +
-                     (kFused ? kFusedLds + size_t(fused_rows(a.k)) * fused_pitch(a.k) : 0);
+  auto kern = linear_rows_kernel<kGated, kExperts, kX, C, MF, U, kOcc>;
+  const size_t lds = size_t(kRowsWaves) * (kGated ? 2 : 1) * C * MF * 1024 +
+                     (kX ? kFusedLds + size_t(fused_rows(a.k, kX)) * fused_pitch(a.k) : 0);
   static LdsLimit limit;
   if (const int rc = limit.raise(kern, lds); rc != I8CONV_OK) return rc;
-  const dim3 grid(unsigned((a.n + 15) / 16), unsigned(kExperts ? std::min(a.experts, a.rows) : 1));
+  const dim3 grid(unsigned((a.n + 16 * C - 1) / (16 * C)), unsigned(kExperts ? std::min(a.experts, a.rows) : 1));
   I8_LAUNCH(kern, grid, dim3(kRowsThreads), lds, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
@@ -318,18 +318,41 @@ int launch_rows(const LinearArgs &a, hipStream_t s) {
 
 template <bool kGated, bool kExperts>
 int launch_any(const LinearArgs &a, bool fused, hipStream_t s) {
-  if (fused) return launch_rows<kGated, kExperts, true, 1, 8>(a, s);
-  if (kExperts || a.rows <= 16) return launch_rows<kGated, kExperts, false, 1, 8>(a, s);
-  if (a.rows <= 32) return launch_rows<kGated, kExperts, false, 2, 4>(a, s);
-  return launch_rows<kGated, kExperts, false, 4, 4>(a, s);
+  // 32 channels to a workgroup where they are so many that several rounds of
+  // them follow: 8 rows of 8 experts 1024 -> 2048, 8.4 us against 13.6 with 16
+  // channels; 148 rows of 60 experts 720 -> 1040, 8.7 and 9.5; one row 4096 ->
+  // 4096 (256 workgroups of 16), 10.0 and 8.6.  Gated ones read twice the
+  // weights and stay at 16 (12288 outputs of 4096, 16 rows: 31.9 and 27.5).
+  constexpr bool kWideToo = !kGated;
+  const int64_t groups = kExperts ? std::min(a.experts, a.rows) : 1;
+  const bool wide = kWideToo && (int64_t(a.n) + 15) / 16 * groups >= 1024;
+  constexpr int C = kWideToo ? 2 : 1;
+  if (fused) {
+    constexpr int U = kGated ? 4 : 8;
+    if (a.x_type == I8CONV_FP32)
+      return wide ? launch_rows<kGated, kExperts, 4, C, 1, U / C, 4>(a, s)
+                  : launch_rows<kGated, kExperts, 4, 1, 1, U, 4>(a, s);
+    return wide ? launch_rows<kGated, kExperts, 2, C, 1, U / C, 4>(a, s)
+                : launch_rows<kGated, kExperts, 2, 1, 1, U, 4>(a, s);
+  }
+  if (kExperts || a.rows <= 16) {
+    constexpr int U = kGated ? 2 : 4;
+    return wide ? launch_rows<kGated, kExperts, 0, C, 1, U, 8 - C>(a, s)
+                : launch_rows<kGated, kExperts, 0, 1, 1, U, 8>(a, s);
+  }
+  if constexpr (!kExperts) {
+    if (a.rows <= 32) return launch_rows<kGated, false, 0, 1, 2, 4, 4>(a, s);
+    return launch_rows<kGated, false, 0, 1, 4, 4, 2>(a, s);
+  }
+  return I8CONV_BAD_ARGUMENT;  // not reached
 }
 
 }  // namespace
 
 // Rows that a workgroup quantizes itself at a time.
-int fused_rows(int k) {
+int fused_rows(int k, int size) {
   const int chunks = (k + 8 * kRowsThreads - 1) / (8 * kRowsThreads);
-  return chunks > kFusedChunks ? 0 : kFusedChunks / chunks;
+  return fused_chunks(size) / chunks;
 }
 
 int launch_linear_rows(const LinearArgs &a, bool gated, bool fused, void *stream) {

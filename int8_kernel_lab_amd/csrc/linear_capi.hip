@@ -93,8 +93,9 @@ RowsPlan plan_rows(const i8conv_linear_shape &s, const void *input) {
   p.few = s.experts ? rows <= 4 * s.experts : rows <= 64;
   p.fused = p.few && s.input_type != I8CONV_INT8 && aligned(input, 16) &&
             ld * type_size(s.input_type) % 16 == 0 &&
-            (s.experts ? std::min(rows, s.rows) : rows) <= 16 && fused_rows(s.inputs) > 0 &&
-            (s.experts ? rows <= 2 * s.experts : rows <= fused_rows(s.inputs));
+            (s.experts ? std::min(rows, s.rows) : rows) <= 16 && fused_rows(s.inputs, type_size(s.input_type)) > 0 &&
+            (s.experts ? rows <= 2 * s.experts
+                       : rows <= fused_rows(s.inputs, type_size(s.input_type)));
   return p;
 }
 
@@ -225,8 +226,8 @@ int i8conv_quantize_rows(const void *input, int type, int32_t rows, int32_t inpu
 }
 
 size_t i8conv_route_workspace_bytes(const i8conv_route_shape *shape) {
-  (void)shape;
-  return 0;
+  if (check_route(shape) != I8CONV_OK) return 0;
+  return route_workspace(int64_t(shape->tokens) * shape->choices, shape->experts);
 }
 
 int i8conv_launch_route(const i8conv_route_shape *shape, const int32_t *ids, int32_t *offsets,
@@ -234,14 +235,17 @@ int i8conv_launch_route(const i8conv_route_shape *shape, const int32_t *ids, int
                         void *stream) {
   const int rc = check_route(shape);
   if (rc != I8CONV_OK) return rc;
-  (void)workspace;
-  (void)workspace_size;
   if (!offsets || (shape->tokens > 0 && (!ids || !sources || !places)))
     return fail(I8CONV_BAD_ARGUMENT, "route: null tensor pointer");
   if (!aligned(ids, 4) || !aligned(offsets, 4) || !aligned(sources, 4) || !aligned(places, 4))
     return fail(I8CONV_BAD_ARGUMENT, "route: tensors must be 4-byte aligned");
+  const size_t need = i8conv_route_workspace_bytes(shape);
+  if (need && (!workspace || workspace_size < need || !aligned(workspace, 256))) {
+    set_error("route: needs a 256-byte aligned workspace of " + std::to_string(need) + " bytes");
+    return I8CONV_WORKSPACE_TOO_SMALL;
+  }
   return launch_route(ids, shape->tokens, shape->choices, shape->experts, offsets, sources, places,
-                      stream);
+                      workspace, stream);
 }
 
 int i8conv_launch_combine(const i8conv_combine_shape *shape, const void *input,
