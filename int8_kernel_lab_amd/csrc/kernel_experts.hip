@@ -115,12 +115,14 @@ __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(
   // expert threadIdx.x (experts <= kRouteThreads): its rows before this part and in all
   const int e = threadIdx.x;
   int before = 0, all = 0;
-  if (e < experts)
+  if (e < experts) {
+#pragma unroll 8
     for (int p = 0; p < parts; ++p) {
       const int c = counts[int64_t(p) * experts + e];
       before += p < part ? c : 0;
       all += c;
     }
+  }
   int sum = all;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -175,8 +177,9 @@ __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(
 // A token's rows are read four at a time, eight values of 16 bits or four of 32
 // per thread (kVec; else single ones).
 template <bool kVec, int V>
-__global__ __launch_bounds__(kThreads) void combine_kernel(const void *x, const int32_t *places,
-                                                           const float *weights,
+__global__ __launch_bounds__(kThreads) void combine_kernel(const void *x,
+                                                           const int32_t *__restrict__ places,
+                                                           const float *__restrict__ weights,
                                                            const void *residual, void *y,
                                                            int64_t tokens, int choices, int n,
                                                            int rows, int in_type, int out_type) {

@@ -62,8 +62,7 @@ constexpr int kRowGroup = 8;
 // stage buffers of its own, take the k-stages in turn and add their sums up
 // through LDS; fragments read GS k-steps of 32 bytes at a time.
 template <int BM, int BN, int WM, int WN, int R, int KG, int GS, int kOcc, bool kGated, bool kExperts>
-__global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearArgs a,
-                                                                        int tiles_m_max) {
+__global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearArgs a) {
   constexpr int P = kStageBytes, KS = P / 32, RPC = 1024 / P;
   constexpr int kWaves = WM * WN;
   constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
@@ -82,40 +81,69 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
   const int lane = threadIdx.x & 63;
   const int wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = wave_id / kWaves, wave = wave_id % kWaves;
-  const int wm = wave % WM, wn = wave / WM;
+  // (waves of different rows share a SIMD, so that one gains by the other's rest)
+  const int wm = wave / WN, wn = wave % WN;
   int8_t *const bufs = smem + group * R * kTile;
   const uint32_t lds0 = lds_addr(bufs);
   float *const params = reinterpret_cast<float *>(smem + KG * R * kTile);  // two slots
-  int *const first = reinterpret_cast<int *>(params + 2 * kParams);  // by expert: its first row tile
+  // by expert: its first whole row tile, and its rank among the experts whose
+  // rows end in a part of one
+  int *const first = reinterpret_cast<int *>(params + 2 * kParams);
+  uint16_t *const ends = reinterpret_cast<uint16_t *>(first + a.experts + 1);
   // stages per group (the last ones may lie past the reduction: zeros)
   const int stages = (a.k + KG * P - 1) / (KG * P);
   const int tiles_n = (a.n + BO - 1) / BO;
   const bool gather = kExperts && a.sources != nullptr;
 
-  int tiles_m = tiles_m_max;
+  // By expert: all whole row tiles first, then the parts, which cost less: the
+  // last round is one of them.
+  int whole = (a.rows + BM - 1) / BM, parts = 0;
   if constexpr (kExperts) {
-    // first[e] = row tiles of the experts before e (one wave, 64 at a time)
     if (wave_id == 0) {
-      int total = 0;
+      int tiles = 0, rests = 0;
       for (int e0 = 0; e0 < a.experts; e0 += 64) {
         const int e = e0 + lane;
-        int count = 0;
-        if (e < a.experts) count = (max(0, a.offsets[e + 1] - a.offsets[e]) + BM - 1) / BM;
-        int sum = count;
+        const int count = e < a.experts ? min(max(0, a.offsets[e + 1] - a.offsets[e]), a.rows) : 0;
+        int sum = count / BM;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
           const int up = __shfl_up(sum, d);
           sum += lane >= d ? up : 0;
         }
-        if (e < a.experts) first[e] = total + sum - count;
-        total += __shfl(sum, 63);
+        const uint64_t rest = __ballot(count % BM != 0);
+        if (e < a.experts) {
+          first[e] = tiles + sum - count / BM;
+          ends[e] = uint16_t(rests + __popcll(rest & ((uint64_t(1) << lane) - 1)));
+        }
+        tiles += __shfl(sum, 63);
+        rests += __popcll(rest);
       }
-      if (lane == 0) first[a.experts] = total;
+      if (lane == 0) {
+        first[a.experts] = tiles;
+        ends[a.experts] = uint16_t(rests);
+      }
     }
     __syncthreads();
-    tiles_m = __builtin_amdgcn_readfirstlane(min(tiles_m_max, first[a.experts]));
+    whole = __builtin_amdgcn_readfirstlane(min(a.rows / BM, first[a.experts]));
+    parts = __builtin_amdgcn_readfirstlane(int(ends[a.experts]));
   }
-  const TileRun run = xcd_tile_run(tiles_m * tiles_n, int(gridDim.x), int(blockIdx.x));
+  // The second run begins at the other end of the XCD's workgroups: those that
+  // got a tile less in the first get one more in it.
+  TileRun run = xcd_tile_run(whole * tiles_n, int(gridDim.x), int(blockIdx.x));
+  int t = run.first;
+  bool in_parts = false;
+  auto skip_empty = [&]() {  // false: no tile is left
+    if constexpr (kExperts) {
+      if (t >= run.last && !in_parts) {
+        const int xcds = gridDim.x >= 8 ? 8 : 1, xcd = int(blockIdx.x) % xcds;
+        const int other = (run.step - 1 - int(blockIdx.x) / xcds) * xcds + xcd;
+        run = xcd_tile_run(parts * tiles_n, int(gridDim.x), other);
+        t = run.first;
+        in_parts = true;
+      }
+    }
+    return t < run.last;
+  };
 
   // copies: this lane's row within a copy's eight and its chunk of the row
   const int crow = lane / (P / 16);
@@ -137,6 +165,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
   // inside the tensors: their sums go nowhere.  Chunks past k have to be zero
   // in one operand, and are in x.
   auto setup = [&](int t) {
+    const int tiles_m = in_parts ? parts : whole;
     const int in_group = kRowGroup * tiles_n, g = t / in_group, m0 = g * kRowGroup;
     const int gm = min(kRowGroup, tiles_m - m0), at = t - g * in_group;
     const int tm = m0 + at % gm;
@@ -144,18 +173,20 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
     row0 = tm * BM;
     int row_end = a.rows;
     if constexpr (kExperts) {
-      int lo = 0, hi = a.experts;  // the last e with first[e] <= tm
+      auto begin_of = [&](int e) { return in_parts ? int(ends[e]) : first[e]; };
+      int lo = 0, hi = a.experts;  // the last e with begin_of(e) <= tm
       while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (first[mid] <= tm)
+        if (begin_of(mid) <= tm)
           lo = mid;
         else
           hi = mid;
       }
       expert = __builtin_amdgcn_readfirstlane(lo);
-      const int begin = a.offsets[expert];
-      row0 = __builtin_amdgcn_readfirstlane(begin + (tm - first[expert]) * BM);
-      row_end = __builtin_amdgcn_readfirstlane(min(a.offsets[expert + 1], a.rows));
+      const int begin = a.offsets[expert], end = min(a.offsets[expert + 1], a.rows);
+      const int tile = in_parts ? (end - begin) / BM : tm - first[expert];
+      row0 = __builtin_amdgcn_readfirstlane(begin + tile * BM);
+      row_end = __builtin_amdgcn_readfirstlane(end);
       if (row0 < 0) row0 = row_end = 0;  // offsets that are no offsets
     }
     rows = max(0, min(BM, row_end - row0));
@@ -229,8 +260,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
     }
   };
 
-  int t = run.first;
-  if (t >= run.last) return;
+  if (!skip_empty()) return;
   setup(t);
   int slot = 0;
   bool later = false;  // a tile after the first: stores may follow its copies
@@ -264,9 +294,25 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
         fb[set.value][ks][n - FN] = *reinterpret_cast<const v4i *>(p + bbuf + 32 * P * (n - FN));
     };
     constexpr int kMfma = GS * FN * FM, kReads = GS * (FN + FM);
-#pragma unroll
-    for (int q = 0; q < kReads; ++q) read(Set<0>{}, bufs, 0, q);
     int ring = 0;
+    // a wave whose rows all lie past the tile's last only copies
+    const bool idle = FM * FN >= 4 && wm * TM >= rows;
+    if (idle) {
+      for (int s = 0; s < stages; ++s) {
+        if (s + R <= stages)
+          wait_vm<(R - 2) * CPW>();
+        else if (s + 1 < stages)
+          wait_vm<0>();
+        barrier_lds();
+        if (s + R < stages) {
+#pragma unroll
+          for (int q = 0; q < CPW; ++q) copy(s + R, ring, q);
+        }
+        ring = ring + 1 == R ? 0 : ring + 1;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < kReads; ++q) read(Set<0>{}, bufs, 0, q);
     for (int s = 0; s < stages; ++s) {
       const int8_t *const buf = bufs + ring * kTile;
       const int next = ring + 1 == R ? 0 : ring + 1;
@@ -305,11 +351,12 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
       part(Set<1>{}, std::true_type{}, NP - 1);
       ring = next;
     }
+    }
 
     const int out_n = n0, out_row = row0, out_rows = rows;
     const float *const pr = params + slot * kParams;
     t += run.step;
-    const bool again = t < run.last;
+    const bool again = skip_empty();
 
     // Outputs of rows 8 g + 4 (lane / 32) + e of the wave's output block i (kPair:
     // of i and i + 1), row block j, from the lane's sums of quad g (all in 32 bits)
@@ -438,7 +485,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
       // 8192, 434 us; 270 with one output type's code only.)
       constexpr int U = 4 / Q, kSteps = FM * (FO / B) * U;
 #pragma unroll 1
-      for (int st = 0; st < kSteps; ++st) {
+      for (int st = idle ? kSteps : 0; st < kSteps; ++st) {
         v4i sg[B][Q], su[B][Q];
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
@@ -513,7 +560,7 @@ template <int BM, int BN, int WM, int WN, int R, int KG, int GS, int kOcc, int k
 int launch_tile(const LinearArgs &a, hipStream_t s) {
   auto kern = linear_kernel<BM, BN, WM, WN, R, KG, GS, kOcc, kGated, kExperts>;
   const size_t lds = size_t(KG) * R * (BM + BN) * kStageBytes + 2 * size_t(2 * BN + BM) * 4 +
-                     (kExperts ? size_t(a.experts + 1) * 4 : 0);
+                     (kExperts ? size_t(a.experts + 1) * 6 : 0);
   constexpr int BO = kGated ? BN / 2 : BN;
   // by expert: every group may end in a part of a tile
   int64_t tiles_m = (int64_t(a.rows) + BM - 1) / BM;
@@ -522,7 +569,7 @@ int launch_tile(const LinearArgs &a, hipStream_t s) {
   static LdsLimit limit;
   if (const int rc = limit.raise(kern, lds); rc != I8CONV_OK) return rc;
   I8_LAUNCH(kern, dim3(unsigned(std::min<int64_t>(tiles, 256 * kGroups))), dim3(64 * WM * WN * KG), lds,
-            s, a, int(tiles_m));
+            s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
     set_error(std::string("linear kernel launch: ") + hipGetErrorString(e));

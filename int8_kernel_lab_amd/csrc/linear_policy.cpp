@@ -1,6 +1,7 @@
 // Which kernel runs an int8 linear layer: the policy of the linear layers, kept
 // outside the kernels like that of the convolutions (policy.cpp).
 #include <algorithm>
+#include <cmath>
 
 #include "i8conv_internal.hpp"
 #include "linear_common.hpp"
@@ -29,16 +30,17 @@ const TileCost kTiles[] = {
     {kTile128x64Pair, 128, 64, 1, 2, false, true, 0.60, 0.76, 2.5},
 };
 
-double cost(const TileCost &t, int64_t row_tiles, int64_t wide, int64_t k) {
-  const int64_t tiles = row_tiles * ((wide + t.bn - 1) / t.bn);
-  const int64_t slots = 256 * t.per_unit, rounds = tiles / slots, rest = tiles % slots;
+// Whole tiles and parts of one (which take about kPart of one's time) as rounds
+// of the chip, the last of them as full as it is.
+constexpr double kPart = 0.65;
+
+double cost(const TileCost &t, double row_tiles, int64_t wide, int64_t k) {
+  const double tiles = row_tiles * double((wide + t.bn - 1) / t.bn);
+  const double slots = 256.0 * t.per_unit, rounds = std::floor(tiles / slots);
+  const double fill = tiles / slots - rounds;
   const double stages = double((k + 128 * t.kg - 1) / (128 * t.kg));
-  double us = double(rounds) * (stages * t.full + t.besides);
-  if (rest) {
-    // the last round: how full its compute units are
-    const double fill = double(rest) / double(slots);
-    us += stages * (t.alone + (t.full - t.alone) * fill) + t.besides;
-  }
+  double us = rounds * (stages * t.full + t.besides);
+  if (fill > 0) us += stages * (t.alone + (t.full - t.alone) * fill) + t.besides;
   return us;
 }
 
@@ -49,9 +51,12 @@ int plan_linear_tile(int64_t rows, int64_t experts, int64_t n, int64_t k, bool g
   double least = 1e300;
   for (const TileCost &t : kTiles) {
     if (gated ? !t.gated : !t.plain) continue;
-    int64_t row_tiles = (rows + t.bm - 1) / t.bm;
-    // by expert: each group ends in a part of a tile, in the mean half of one
-    if (experts) row_tiles = rows / t.bm + (std::min(experts, rows) + 1) / 2;
+    double row_tiles = double((rows + t.bm - 1) / t.bm);
+    if (experts) {
+      // each group ends in a part of a tile, in the mean half of one
+      const double groups = double(std::min(experts, rows));
+      row_tiles = std::max(0.0, double(rows) / t.bm - groups / 2) + kPart * groups;
+    }
     const double us = cost(t, row_tiles, gated ? 2 * n : n, k);
     if (us < least) least = us, best = t.tile;
   }
