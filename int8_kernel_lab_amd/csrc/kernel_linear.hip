@@ -86,64 +86,46 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
   int8_t *const bufs = smem + group * R * kTile;
   const uint32_t lds0 = lds_addr(bufs);
   float *const params = reinterpret_cast<float *>(smem + KG * R * kTile);  // two slots
-  // by expert: its first whole row tile, and its rank among the experts whose
-  // rows end in a part of one
-  int *const first = reinterpret_cast<int *>(params + 2 * kParams);
-  uint16_t *const ends = reinterpret_cast<uint16_t *>(first + a.experts + 1);
+  // by expert: its first row and its first row tile
+  int *const begins = reinterpret_cast<int *>(params + 2 * kParams);
+  int *const first = begins + a.experts + 1;
   // stages per group (the last ones may lie past the reduction: zeros)
   const int stages = (a.k + KG * P - 1) / (KG * P);
   const int tiles_n = (a.n + BO - 1) / BO;
   const bool gather = kExperts && a.sources != nullptr;
 
-  // By expert: all whole row tiles first, then the parts, which cost less: the
-  // last round is one of them.
-  int whole = (a.rows + BM - 1) / BM, parts = 0;
+  int tiles_m = (a.rows + BM - 1) / BM;
   if constexpr (kExperts) {
+    // first[e] = row tiles of the experts before e (one wave, 64 at a time)
     if (wave_id == 0) {
-      int tiles = 0, rests = 0;
+      int total = 0;
       for (int e0 = 0; e0 < a.experts; e0 += 64) {
         const int e = e0 + lane;
-        const int count = e < a.experts ? min(max(0, a.offsets[e + 1] - a.offsets[e]), a.rows) : 0;
-        int sum = count / BM;
+        int count = 0;
+        if (e < a.experts) {
+          const int begin = a.offsets[e], end = a.offsets[e + 1];
+          count = min(max(0, end - begin), a.rows);
+          count = count / BM + (count % BM != 0);
+          begins[e] = begin;
+          if (e + 1 == a.experts) begins[a.experts] = end;
+        }
+        int sum = count;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
           const int up = __shfl_up(sum, d);
           sum += lane >= d ? up : 0;
         }
-        const uint64_t rest = __ballot(count % BM != 0);
-        if (e < a.experts) {
-          first[e] = tiles + sum - count / BM;
-          ends[e] = uint16_t(rests + __popcll(rest & ((uint64_t(1) << lane) - 1)));
-        }
-        tiles += __shfl(sum, 63);
-        rests += __popcll(rest);
+        if (e < a.experts) first[e] = total + sum - count;
+        total += __shfl(sum, 63);
       }
-      if (lane == 0) {
-        first[a.experts] = tiles;
-        ends[a.experts] = uint16_t(rests);
-      }
+      if (lane == 0) first[a.experts] = total;
     }
     __syncthreads();
-    whole = __builtin_amdgcn_readfirstlane(min(a.rows / BM, first[a.experts]));
-    parts = __builtin_amdgcn_readfirstlane(int(ends[a.experts]));
+    // (no more than there can be, whatever the offsets say)
+    tiles_m = __builtin_amdgcn_readfirstlane(
+        min(first[a.experts], a.rows / BM + min(a.experts, a.rows)));
   }
-  // The second run begins at the other end of the XCD's workgroups: those that
-  // got a tile less in the first get one more in it.
-  TileRun run = xcd_tile_run(whole * tiles_n, int(gridDim.x), int(blockIdx.x));
-  int t = run.first;
-  bool in_parts = false;
-  auto skip_empty = [&]() {  // false: no tile is left
-    if constexpr (kExperts) {
-      if (t >= run.last && !in_parts) {
-        const int xcds = gridDim.x >= 8 ? 8 : 1, xcd = int(blockIdx.x) % xcds;
-        const int other = (run.step - 1 - int(blockIdx.x) / xcds) * xcds + xcd;
-        run = xcd_tile_run(parts * tiles_n, int(gridDim.x), other);
-        t = run.first;
-        in_parts = true;
-      }
-    }
-    return t < run.last;
-  };
+  const TileRun run = xcd_tile_run(tiles_m * tiles_n, int(gridDim.x), int(blockIdx.x));
 
   // copies: this lane's row within a copy's eight and its chunk of the row
   const int crow = lane / (P / 16);
@@ -165,7 +147,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
   // inside the tensors: their sums go nowhere.  Chunks past k have to be zero
   // in one operand, and are in x.
   auto setup = [&](int t) {
-    const int tiles_m = in_parts ? parts : whole;
     const int in_group = kRowGroup * tiles_n, g = t / in_group, m0 = g * kRowGroup;
     const int gm = min(kRowGroup, tiles_m - m0), at = t - g * in_group;
     const int tm = m0 + at % gm;
@@ -173,20 +154,17 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
     row0 = tm * BM;
     int row_end = a.rows;
     if constexpr (kExperts) {
-      auto begin_of = [&](int e) { return in_parts ? int(ends[e]) : first[e]; };
-      int lo = 0, hi = a.experts;  // the last e with begin_of(e) <= tm
+      int lo = 0, hi = a.experts;  // the last e with first[e] <= tm
       while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (begin_of(mid) <= tm)
+        if (first[mid] <= tm)
           lo = mid;
         else
           hi = mid;
       }
       expert = __builtin_amdgcn_readfirstlane(lo);
-      const int begin = a.offsets[expert], end = min(a.offsets[expert + 1], a.rows);
-      const int tile = in_parts ? (end - begin) / BM : tm - first[expert];
-      row0 = __builtin_amdgcn_readfirstlane(begin + tile * BM);
-      row_end = __builtin_amdgcn_readfirstlane(end);
+      row0 = __builtin_amdgcn_readfirstlane(begins[expert] + (tm - first[expert]) * BM);
+      row_end = __builtin_amdgcn_readfirstlane(min(begins[expert + 1], a.rows));
       if (row0 < 0) row0 = row_end = 0;  // offsets that are no offsets
     }
     rows = max(0, min(BM, row_end - row0));
@@ -260,7 +238,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
     }
   };
 
-  if (!skip_empty()) return;
+  int t = run.first;
+  if (t >= run.last) return;
   setup(t);
   int slot = 0;
   bool later = false;  // a tile after the first: stores may follow its copies
@@ -356,7 +335,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
     const int out_n = n0, out_row = row0, out_rows = rows;
     const float *const pr = params + slot * kParams;
     t += run.step;
-    const bool again = skip_empty();
+    const bool again = t < run.last;
 
     // Outputs of rows 8 g + 4 (lane / 32) + e of the wave's output block i (kPair:
     // of i and i + 1), row block j, from the lane's sums of quad g (all in 32 bits)
@@ -560,7 +539,7 @@ template <int BM, int BN, int WM, int WN, int R, int KG, int GS, int kOcc, int k
 int launch_tile(const LinearArgs &a, hipStream_t s) {
   auto kern = linear_kernel<BM, BN, WM, WN, R, KG, GS, kOcc, kGated, kExperts>;
   const size_t lds = size_t(KG) * R * (BM + BN) * kStageBytes + 2 * size_t(2 * BN + BM) * 4 +
-                     (kExperts ? size_t(a.experts + 1) * 6 : 0);
+                     (kExperts ? size_t(a.experts + 1) * 8 : 0);
   constexpr int BO = kGated ? BN / 2 : BN;
   // by expert: every group may end in a part of a tile
   int64_t tiles_m = (int64_t(a.rows) + BM - 1) / BM;

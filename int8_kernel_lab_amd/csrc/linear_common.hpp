@@ -107,24 +107,25 @@ __device__ __forceinline__ void store_values4(void *p, int64_t i, int type, v4f 
 
 // The activation of N values, of a wave-uniform kind.  relu keeps NaN.
 // gelu_tanh and silu are both v times the logistic function of a polynomial:
-// 0.5 (1 + tanh(z / 2)) = 1 / (1 + exp(-z)); their exponentials overflow to
-// infinity for large negative values and the product is then -0, the limit.
+// 0.5 (1 + tanh(z / 2)) = 1 / (1 + 2^(-z log2 e)); their exponentials overflow
+// to infinity for large negative values and the product is then -0, the limit.
 template <int N>
 __device__ __forceinline__ void activate(float (&v)[N], int kind) {
-  if (kind <= I8CONV_ACT_RELU) {
-    const float floor = kind == I8CONV_ACT_RELU ? 0.0f : -__builtin_inff();
+  if (kind == I8CONV_ACT_NONE) return;
+  if (kind == I8CONV_ACT_RELU) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = v[i] < floor ? floor : v[i];
+    for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
   } else if (kind == I8CONV_ACT_GELU) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678f));
   } else {
-    const float c1 = kind == I8CONV_ACT_SILU ? 1.0f : 1.5957691216f;
-    const float c3 = kind == I8CONV_ACT_SILU ? 0.0f : 0.0713548162726f;
+    // -log2 e times 1, or times 2 sqrt(2 / pi) (1, 0.044715)
+    const float c1 = kind == I8CONV_ACT_SILU ? -1.44269504f : -2.30220820f;
+    const float c3 = kind == I8CONV_ACT_SILU ? 0.0f : -0.10294324f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float z = v[i] * fmaf(c3 * v[i], v[i], c1);
-      v[i] *= __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+      v[i] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z));
     }
   }
 }

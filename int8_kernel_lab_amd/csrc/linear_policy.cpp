@@ -15,24 +15,24 @@ namespace {
 // sweeps of 80 to 4096 rows over 1024 to 12288 columns, 1024 to 8192 deep, on
 // all tiles.
 struct TileCost {
-  int tile, bm, bn, per_unit, kg;
+  int tile, bm, bn, per_unit, kg, buffers;
   bool plain, gated;
   double alone, full, besides;
 };
 const TileCost kTiles[] = {
-    {kTile256x256, 256, 256, 1, 1, true, true, 1.25, 1.80, 5.0},
-    {kTile128x256, 128, 256, 1, 1, true, true, 0.76, 1.10, 4.0},
-    {kTile128x128, 128, 128, 2, 1, true, true, 0.66, 1.18, 3.0},
-    {kTile128x64, 128, 64, 3, 1, true, true, 0.60, 1.05, 2.5},
-    {kTile64x64, 64, 64, 4, 1, true, false, 0.50, 0.90, 2.0},
-    {kTile64x64Deep, 64, 64, 2, 1, true, false, 0.28, 0.45, 2.0},
-    {kTile64x64Pair, 64, 64, 1, 2, true, false, 0.42, 0.50, 2.5},
-    {kTile128x64Pair, 128, 64, 1, 2, false, true, 0.60, 0.76, 2.5},
+    {kTile256x256, 256, 256, 1, 1, 2, true, true, 1.25, 1.80, 5.0},
+    {kTile128x256, 128, 256, 1, 1, 3, true, true, 0.76, 1.10, 4.0},
+    {kTile128x128, 128, 128, 2, 1, 2, true, true, 0.66, 1.18, 3.0},
+    {kTile128x64, 128, 64, 3, 1, 2, true, true, 0.60, 1.05, 2.5},
+    {kTile64x64, 64, 64, 4, 1, 2, true, false, 0.50, 0.90, 2.0},
+    {kTile64x64Deep, 64, 64, 2, 1, 4, true, false, 0.28, 0.45, 2.0},
+    {kTile64x64Pair, 64, 64, 1, 2, 4, true, false, 0.42, 0.50, 2.5},
+    {kTile128x64Pair, 128, 64, 1, 2, 3, false, true, 0.60, 0.76, 2.5},
 };
 
 // Whole tiles and parts of one (which take about kPart of one's time) as rounds
 // of the chip, the last of them as full as it is.
-constexpr double kPart = 0.65;
+constexpr double kPart = 0.8;
 
 double cost(const TileCost &t, double row_tiles, int64_t wide, int64_t k) {
   const double tiles = row_tiles * double((wide + t.bn - 1) / t.bn);
@@ -51,6 +51,10 @@ int plan_linear_tile(int64_t rows, int64_t experts, int64_t n, int64_t k, bool g
   double least = 1e300;
   for (const TileCost &t : kTiles) {
     if (gated ? !t.gated : !t.plain) continue;
+    // the LDS of every workgroup of a unit (launch_tile has the same sum)
+    const int64_t lds = int64_t(t.kg) * t.buffers * (t.bm + t.bn) * kStageBytes +
+                        8 * (2 * t.bn + t.bm) + (experts ? 8 * (experts + 1) : 0);
+    if (lds * t.per_unit > kLdsBudget) continue;
     double row_tiles = double((rows + t.bm - 1) / t.bm);
     if (experts) {
       // each group ends in a part of a tile, in the mean half of one
