@@ -264,8 +264,9 @@ typedef enum i8conv_activation {
 
 /* A linear layer.  `rows` may be 0 (nothing is launched).  inputs % 16 == 0
  * and < 2^17; the weights of one matrix (outputs, or 2 * outputs where gated,
- * times inputs) below 2^31 bytes.  Strides are elements between rows, 0 for
- * packed rows; that of an int8 input is a multiple of 16 below 2^23. */
+ * times inputs) below 2^31 bytes, outputs below 2^24.  Strides are elements
+ * between rows, 0 for packed rows; that of an int8 input is a multiple of 16
+ * below 2^23, those of output and residual are below 2^24. */
 typedef struct i8conv_linear_shape {
   int32_t rows;            /* rows of the input (tokens) */
   int32_t inputs, outputs; /* values of a row */

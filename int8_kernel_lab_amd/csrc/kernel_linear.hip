@@ -341,13 +341,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
     // of i and i + 1), row block j, from the lane's sums of quad g (all in 32 bits)
     constexpr int B = kPair ? 2 : 1;
     const int half = lane >> 5;
-    const int size = a.out_type == I8CONV_FP32 ? 4 : 2;
-    const auto yr = make_rsrc(static_cast<int8_t *>(a.y) + int64_t(out_row) * a.ldy * size,
-                              a.vec2 && out_rows ? uint32_t((out_rows - 1) * int(a.ldy) + a.n) * uint32_t(size) : 0u);
-    const auto rr = make_rsrc(static_cast<const int8_t *>(a.residual ? a.residual : a.y) +
-                                  int64_t(out_row) * a.ldr * size,
-                              a.vec2 && out_rows && a.residual
-                                  ? uint32_t((out_rows - 1) * int(a.ldr) + a.n) * uint32_t(size) : 0u);
     // Q quads, from g0 on, of row block j: their sums sg (and su, the other
     // halves'), for each of the B blocks
     constexpr int Q = kGated ? 1 : 2;
@@ -355,6 +348,50 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
       const int ct = wn * (32 * FO) + (kPair ? i * 32 + 2 * (lane & 31) : 32 * i + (lane & 31));
       const int ch = out_n + ct;
       const int r0 = wm * TM + 32 * j + 4 * half + 8 * g0;
+      // windows over this step's rows, its first one at 0: rows past the tile's
+      // last are out of their range, and so is the column of a channel past n
+      const int size = a.out_type == I8CONV_FP32 ? 4 : 2;
+      const int w0 = wm * TM + 32 * j + 8 * g0, left = out_rows - w0;
+      const uint32_t yp = uint32_t(a.ldy) * uint32_t(size), rp = uint32_t(a.ldr) * uint32_t(size);
+      const auto window = [&](const void *base, int64_t ld, uint32_t pitch) {
+        const int in = min(left, 8 * Q);
+        return make_rsrc(static_cast<const int8_t *>(base) + (out_row + w0) * ld * size,
+                         in > 0 && base ? uint32_t(in - 1) * pitch + uint32_t(a.n) * uint32_t(size) : 0u);
+      };
+      const auto yr = window(a.y, a.ldy, yp), rr = window(a.residual, a.ldr, rp);
+      auto row_of = [&](int e) { return 4 * half + 8 * (e / 4) + e % 4; };
+      // 16-bit outputs of single blocks, two channels to a dword: of every two
+      // rows an even lane takes the first and its odd neighbour the second
+      const int odd = kPair ? 0 : lane & 1;
+      constexpr int W = kPair ? 4 * Q : 2 * Q;  // dwords
+      auto word_row = [&](int w) { return kPair ? row_of(w) : row_of(2 * w) + odd; };
+      const uint32_t cw = ch - odd < a.n ? uint32_t(ch - odd) * uint32_t(size) : kOutOfRange;
+      uint32_t cb[B];
+#pragma unroll
+      for (int b = 0; b < B; ++b) cb[b] = ch + b < a.n ? uint32_t(ch + b) * uint32_t(size) : kOutOfRange;
+
+      // the residual, on its way while the sums are worked on
+      uint32_t res[B][4 * Q];
+      if (a.residual) {
+        if (size == 2 && a.vec2) {
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            res[0][w] = __builtin_amdgcn_raw_buffer_load_b32(rr, cw + uint32_t(word_row(w)) * rp, 0, 0);
+        } else if (size == 2) {
+#pragma unroll
+          for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int e = 0; e < 4 * Q; ++e)
+              res[b][e] = __builtin_amdgcn_raw_buffer_load_b16(rr, cb[b] + uint32_t(row_of(e)) * rp, 0, 0);
+        } else {
+#pragma unroll
+          for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int e = 0; e < 4 * Q; ++e)
+              res[b][e] = __builtin_amdgcn_raw_buffer_load_b32(rr, cb[b] + uint32_t(row_of(e)) * rp, 0, 0);
+        }
+      }
+
       float v[B][4 * Q];
 #pragma unroll
       for (int b = 0; b < B; ++b) {
@@ -378,79 +415,57 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
           for (int e = 0; e < 4 * Q; ++e) v[b][e] *= u[e];
         }
       }
-      auto row_of = [&](int e) { return r0 + 8 * (e / 4) + e % 4; };
-      if (!a.vec2) {  // any alignment and stride, an element at a time
-#pragma unroll
-        for (int b = 0; b < B; ++b)
-#pragma unroll
-          for (int e = 0; e < 4 * Q; ++e)
-            if (ch + b < a.n && row_of(e) < out_rows) {
-              const int64_t row = out_row + row_of(e);
-              float o = v[b][e];
-              if (a.residual) o += load_value(a.residual, row * a.ldr + ch + b, a.out_type);
-              store_value(a.y, row * a.ldy + ch + b, a.out_type, o);
-            }
-        return;
-      }
-      // Rows past the tile's last are out of the windows' range, and so is the
-      // column of a channel past n.
-      const uint32_t yp = uint32_t(a.ldy) * uint32_t(size), rp = uint32_t(a.ldr) * uint32_t(size);
-      if (a.out_type == I8CONV_FP32) {
-        const uint32_t c = ch < a.n ? uint32_t(ch) * 4u : kOutOfRange;
-        if (a.residual) {
-#pragma unroll
-          for (int e = 0; e < 4 * Q; ++e) {
-            const uint32_t off = c + uint32_t(row_of(e)) * rp;
-            if constexpr (kPair) {
-              const v2u t = __builtin_amdgcn_raw_buffer_load_b64(rr, off, 0, 0);
-              v[0][e] += bits_f32(t[0]), v[B - 1][e] += bits_f32(t[1]);
-            } else {
-              v[0][e] += bits_f32(__builtin_amdgcn_raw_buffer_load_b32(rr, off, 0, 0));
-            }
-          }
-        }
+      auto store32 = [&]() {
 #pragma unroll
         for (int e = 0; e < 4 * Q; ++e) {
-          const uint32_t off = c + uint32_t(row_of(e)) * yp;
-          if constexpr (kPair)
-            __builtin_amdgcn_raw_buffer_store_b64(v2u{f32_bits(v[0][e]), f32_bits(v[B - 1][e])}, yr, off, 0, 0);
-          else
-            __builtin_amdgcn_raw_buffer_store_b32(f32_bits(v[0][e]), yr, off, 0, 0);
-        }
-        return;
-      }
-      // Two channels of a row in a dword.  Single blocks: of every two rows an
-      // even lane takes the first and its odd neighbour the second.
-      const int odd = kPair ? 0 : lane & 1, chp = ch - odd;
-      const uint32_t c = chp < a.n ? uint32_t(chp) * 2u : kOutOfRange;
-      constexpr int W = kPair ? 4 * Q : 2 * Q;  // dwords
-      float lo[W], hi[W];
+          float o[B];
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        if constexpr (kPair) {
-          lo[w] = v[0][w], hi[w] = v[B - 1][w];
-        } else {
-          const float got = neighbour(odd ? v[0][2 * w] : v[0][2 * w + 1]);
-          lo[w] = odd ? got : v[0][2 * w];
-          hi[w] = odd ? v[0][2 * w + 1] : got;
-        }
-      }
-      auto word_row = [&](int w) { return kPair ? row_of(w) : row_of(2 * w) + odd; };
-      if (a.residual) {
-        uint32_t t[W];
+          for (int b = 0; b < B; ++b) o[b] = a.residual ? v[b][e] + bits_f32(res[b][e]) : v[b][e];
+          const uint32_t row = uint32_t(row_of(e)) * yp;
+          if (kPair && a.vec2) {
+            __builtin_amdgcn_raw_buffer_store_b64(v2u{f32_bits(o[0]), f32_bits(o[B - 1])}, yr, cb[0] + row, 0, 0);
+          } else {
 #pragma unroll
-        for (int w = 0; w < W; ++w)
-          t[w] = __builtin_amdgcn_raw_buffer_load_b32(rr, c + uint32_t(word_row(w)) * rp, 0, 0);
+            for (int b = 0; b < B; ++b)
+              __builtin_amdgcn_raw_buffer_store_b32(f32_bits(o[b]), yr, cb[b] + row, 0, 0);
+          }
+        }
+      };
+      auto store16 = [&](auto kind) {  // (the type once for all, not per value)
+        constexpr int T = decltype(kind)::value;
+        if (!a.vec2) {
+#pragma unroll
+          for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int e = 0; e < 4 * Q; ++e) {
+              const float o = a.residual ? v[b][e] + from_half(res[b][e] & 0xffffu, T) : v[b][e];
+              __builtin_amdgcn_raw_buffer_store_b16(to_half(o, T), yr, cb[b] + uint32_t(row_of(e)) * yp, 0, 0);
+            }
+          return;
+        }
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          lo[w] += from_half(t[w] & 0xffffu, a.out_type);
-          hi[w] += from_half(t[w] >> 16, a.out_type);
+          float lo, hi;
+          if constexpr (kPair) {
+            lo = v[0][w], hi = v[B - 1][w];
+          } else {
+            const float got = neighbour(odd ? v[0][2 * w] : v[0][2 * w + 1]);
+            lo = odd ? got : v[0][2 * w];
+            hi = odd ? v[0][2 * w + 1] : got;
+          }
+          if (a.residual) {
+            lo += from_half(res[0][w] & 0xffffu, T);
+            hi += from_half(res[0][w] >> 16, T);
+          }
+          __builtin_amdgcn_raw_buffer_store_b32(to_halves(lo, hi, T), yr, cw + uint32_t(word_row(w)) * yp, 0, 0);
         }
-      }
-#pragma unroll
-      for (int w = 0; w < W; ++w)
-        __builtin_amdgcn_raw_buffer_store_b32(to_halves(lo[w], hi[w], a.out_type), yr,
-                                              c + uint32_t(word_row(w)) * yp, 0, 0);
+      };
+      if (a.out_type == I8CONV_FP32)
+        store32();
+      else if (a.out_type == I8CONV_BF16)
+        store16(Set<I8CONV_BF16>{});
+      else
+        store16(Set<I8CONV_FP16>{});
     };
     if constexpr (KG == 1) {
       // the next tile's copies go out before this tile's stores
@@ -469,6 +484,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
           if (st != c) continue;
+          asm volatile("" ::: "memory");  // a branch: selects would run through every block's registers
           const int j = c / U % FM, i = c / U / FM * B, g0 = c % U * Q;
 #pragma unroll
           for (int b = 0; b < B; ++b)

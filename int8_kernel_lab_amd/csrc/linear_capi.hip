@@ -45,6 +45,9 @@ int check_shape(const i8conv_linear_shape *s) {
       (s->output_stride != 0 && s->output_stride < s->outputs) ||
       (s->residual_stride != 0 && s->residual_stride < s->outputs))
     return fail(I8CONV_BAD_SHAPE, "linear: a stride below the row's length");
+  if (s->outputs >= kLinearMaxStride || s->output_stride >= kLinearMaxStride ||
+      s->residual_stride >= kLinearMaxStride)
+    return fail(I8CONV_BAD_SHAPE, "linear: outputs and their strides must be below 2^24");
   if (s->input_type == I8CONV_INT8 && (s->input_stride % 16 != 0 || s->input_stride >= 1 << 23))
     return fail(I8CONV_BAD_SHAPE, "linear: the stride of int8 rows is a multiple of 16 below 2^23");
   return I8CONV_OK;
@@ -128,7 +131,7 @@ int run(const i8conv_linear_shape &s, const void *input, const float *input_scal
            (!residual || linear_vec_ok(residual, a.ldr, a.n, size, count));
   };
   a.vec4 = vec_ok(4);
-  a.vec2 = vec_ok(2) && a.ldy < kVec2MaxStride && (!residual || a.ldr < kVec2MaxStride);
+  a.vec2 = vec_ok(2);
   const RowsPlan plan = plan_rows(s, input);
   a.x_type = s.input_type;
   if (plan.fused || s.input_type == I8CONV_INT8) {

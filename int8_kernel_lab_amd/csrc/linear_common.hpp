@@ -36,8 +36,8 @@ inline bool linear_vec_ok(const void *base, int64_t ld, int n, int size, int cou
   return n % count == 0 && ld % count == 0 &&
          (reinterpret_cast<uintptr_t>(base) & uintptr_t(count * size - 1)) == 0;
 }
-// The two-wide form addresses a tile's rows with 32-bit offsets.
-constexpr int64_t kVec2MaxStride = int64_t(1) << 20;
+// Sixteen rows of an output or residual are addressed with 32-bit offsets.
+constexpr int64_t kLinearMaxStride = int64_t(1) << 24;
 
 I8_HD inline int type_size(int type) {
   return type == I8CONV_INT8 ? 1 : type == I8CONV_FP32 ? 4 : 2;
@@ -56,6 +56,7 @@ __device__ __forceinline__ uint16_t to_bf16(float f) {
 }
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint16_t to_fp16(float f) {
   return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
 }
@@ -74,7 +75,7 @@ __device__ __forceinline__ float from_half(uint32_t h, int type) {
 __device__ __forceinline__ uint32_t to_halves(float lo, float hi, int type) {
   if (type == I8CONV_BF16)
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{lo, hi}, v2bf));
-  return uint32_t(to_fp16(lo)) | uint32_t(to_fp16(hi)) << 16;
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{lo, hi}, v2h));
 }
 
 // One value of a row in memory.
