@@ -318,33 +318,36 @@ int launch_rows(const LinearArgs &a, hipStream_t s) {
 
 template <bool kGated, bool kExperts>
 int launch_any(const LinearArgs &a, bool fused, hipStream_t s) {
-  // 32 channels to a workgroup where they are so many that several rounds of
-  // them follow: 8 rows of 8 experts 1024 -> 2048, 8.4 us against 13.6 with 16
-  // channels; 148 rows of 60 experts 720 -> 1040, 8.7 and 9.5; one row 4096 ->
-  // 4096 (256 workgroups of 16), 10.0 and 8.6.  Gated ones read twice the
-  // weights and stay at 16 (12288 outputs of 4096, 16 rows: 31.9 and 27.5).
-  constexpr bool kWideToo = !kGated;
+  // 32 channels to a workgroup where 16 would take more than a round of two
+  // (codes: four) workgroups to a compute unit: one row 4096 -> 12288, 12.9 us
+  // against 16.1; 8 rows of 8 experts 1024 -> 2048, 8.4 and 13.6; codes of 148
+  // rows of 60 experts 720 -> 1040, 8.7 and 9.5; but one row 4096 -> 4096 (256
+  // workgroups of 16), 10.0 and 8.6, codes of 16 rows 4096 -> 12288 (768), 18.7
+  // and 17.9.  Gated ones read twice the weights and stay at 16 channels: 12288
+  // outputs of 4096, one row 29.5 and 27.9, 16 rows 31.9 and 27.5.
   const int64_t groups = kExperts ? std::min(a.experts, a.rows) : 1;
-  const bool wide = kWideToo && (int64_t(a.n) + 15) / 16 * groups >= 1024;
-  constexpr int C = kWideToo ? 2 : 1;
+  const int64_t narrow = (int64_t(a.n) + 15) / 16 * groups;
   if (fused) {
     constexpr int U = kGated ? 4 : 8;
-    if (a.x_type == I8CONV_FP32)
-      return wide ? launch_rows<kGated, kExperts, 4, C, 1, U / C, 4>(a, s)
-                  : launch_rows<kGated, kExperts, 4, 1, 1, U, 4>(a, s);
-    return wide ? launch_rows<kGated, kExperts, 2, C, 1, U / C, 4>(a, s)
-                : launch_rows<kGated, kExperts, 2, 1, 1, U, 4>(a, s);
+    if constexpr (!kGated) {
+      if (narrow > 512)
+        return a.x_type == I8CONV_FP32 ? launch_rows<false, kExperts, 4, 2, 1, U / 2, 4>(a, s)
+                                       : launch_rows<false, kExperts, 2, 2, 1, U / 2, 4>(a, s);
+    }
+    return a.x_type == I8CONV_FP32 ? launch_rows<kGated, kExperts, 4, 1, 1, U, 4>(a, s)
+                                   : launch_rows<kGated, kExperts, 2, 1, 1, U, 4>(a, s);
   }
   if (kExperts || a.rows <= 16) {
-    constexpr int U = kGated ? 2 : 4;
-    return wide ? launch_rows<kGated, kExperts, 0, C, 1, U, 8 - C>(a, s)
-                : launch_rows<kGated, kExperts, 0, 1, 1, U, 8>(a, s);
+    if constexpr (!kGated) {
+      if (narrow >= 1024) return launch_rows<false, kExperts, 0, 2, 1, 4, 6>(a, s);
+    }
+    return launch_rows<kGated, kExperts, 0, 1, 1, kGated ? 2 : 4, 8>(a, s);
   }
   if constexpr (!kExperts) {
     if (a.rows <= 32) return launch_rows<kGated, false, 0, 1, 2, 4, 4>(a, s);
-    return launch_rows<kGated, false, 0, 1, 4, 4, 2>(a, s);
   }
-  return I8CONV_BAD_ARGUMENT;  // not reached
+  set_error("linear: too many rows for the few-row kernel");
+  return I8CONV_BAD_ARGUMENT;
 }
 
 }  // namespace

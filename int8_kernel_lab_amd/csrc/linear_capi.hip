@@ -84,21 +84,34 @@ int check_tensors(const i8conv_linear_shape &s, const void *input, const float *
   return I8CONV_OK;
 }
 
-// Which kernel runs a layer.
+// Which kernel runs a layer: few rows go through kernel_linear_rows.hip, the
+// fewest of them as they are (it quantizes them itself).  In us with the
+// quantizing launch where there is one, 4096 -> 4096: 16 rows 11.1 and tiles
+// 12.6, 32 rows 13.0 and 12.9, 64 rows 16.5 and 13.1; gated 32 rows 16.4 and
+// 16.4.  64 experts 2048 -> 1024 with half a row each 15.0 and 15.4, two rows
+// 22.2 and 23.3, 1024 -> 2000 18.7 and 15.1, 27.6 and 22.7 (16 experts with a
+// row each 11.5 and 12.1); gated two rows 38.6
+// and 47.8, four 53.4 and 59.6, eight 70.1 and 62.4.  Quantizing in the kernel,
+// 4096 -> 4096: 2 rows 9.0 against 9.8, 4 rows 10.8 and 10.3; 16 experts 2048 ->
+// 1024: 4 rows in all 7.0 and 7.8, gated 8.5 and 10.3, 16 rows 10.9 and 11.2,
+// gated 14.7 and 13.9.
 struct RowsPlan {
-  bool few;    // kernel_linear_rows.hip instead of the tiles
-  bool fused;  // ... which quantizes the rows itself
+  bool few, fused;
 };
 RowsPlan plan_rows(const i8conv_linear_shape &s, const void *input) {
   RowsPlan p{};
-  const int rows = s.experts ? s.routed : s.rows;
+  const int64_t rows = s.experts ? s.routed : s.rows;
   const int64_t ld = s.input_stride ? s.input_stride : s.inputs;
-  p.few = s.experts ? rows <= 4 * s.experts : rows <= 64;
-  p.fused = p.few && s.input_type != I8CONV_INT8 && aligned(input, 16) &&
-            ld * type_size(s.input_type) % 16 == 0 &&
-            (s.experts ? std::min(rows, s.rows) : rows) <= 16 && fused_rows(s.inputs, type_size(s.input_type)) > 0 &&
-            (s.experts ? rows <= 2 * s.experts
-                       : rows <= fused_rows(s.inputs, type_size(s.input_type)));
+  const int size = type_size(s.input_type);
+  if (!s.experts)
+    p.few = rows <= 32;
+  else if (s.gated)
+    p.few = rows <= 4 * int64_t(s.experts);
+  else  // (many short workgroups: tiles sooner)
+    p.few = rows <= 3 * int64_t(s.experts) && std::min<int64_t>(rows, s.experts) * s.outputs <= 1 << 16;
+  const int at_once = fused_rows(s.inputs, size);
+  p.fused = p.few && s.input_type != I8CONV_INT8 && aligned(input, 16) && ld * size % 16 == 0 &&
+            (s.experts ? rows <= 8 && at_once > 0 : rows <= std::min(2, at_once));
   return p;
 }
 
