@@ -343,7 +343,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
     const int half = lane >> 5;
     // Q quads, from g0 on, of row block j: their sums sg (and su, the other
     // halves'), for each of the B blocks
-    constexpr int Q = kGated ? 1 : 2;
+    constexpr int Q = kGated || kOcc == 3 ? 1 : 2;  // (two spill there)
     auto finish = [&](int i, int j, int g0, const v4i (&sg)[B][Q], const v4i (&su)[B][Q]) {
       const int ct = wn * (32 * FO) + (kPair ? i * 32 + 2 * (lane & 31) : 32 * i + (lane & 31));
       const int ch = out_n + ct;
@@ -360,12 +360,16 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
       };
       const auto yr = window(a.y, a.ldy, yp), rr = window(a.residual, a.ldr, rp);
       auto row_of = [&](int e) { return 4 * half + 8 * (e / 4) + e % 4; };
-      // 16-bit outputs of single blocks, two channels to a dword: of every two
-      // rows an even lane takes the first and its odd neighbour the second
-      const int odd = kPair ? 0 : lane & 1;
+      // 16-bit outputs leave two channels to a dword, at any alignment (buffer
+      // accesses need none).  Single blocks: of every two rows an even lane takes
+      // the first and its odd neighbour the second.  With n odd the last channel
+      // is alone.
+      const int odd = kPair ? 0 : lane & 1, pair = ch - odd;
       constexpr int W = kPair ? 4 * Q : 2 * Q;  // dwords
       auto word_row = [&](int w) { return kPair ? row_of(w) : row_of(2 * w) + odd; };
-      const uint32_t cw = ch - odd < a.n ? uint32_t(ch - odd) * uint32_t(size) : kOutOfRange;
+      const uint32_t cw = pair + 1 < a.n ? uint32_t(pair) * uint32_t(size) : kOutOfRange;
+      const uint32_t alone = pair + 1 == a.n ? uint32_t(pair) * uint32_t(size) : kOutOfRange;
+      const bool any_alone = __builtin_amdgcn_ballot_w64(alone != kOutOfRange) != 0;
       uint32_t cb[B];
 #pragma unroll
       for (int b = 0; b < B; ++b) cb[b] = ch + b < a.n ? uint32_t(ch + b) * uint32_t(size) : kOutOfRange;
@@ -373,16 +377,15 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
       // the residual, on its way while the sums are worked on
       uint32_t res[B][4 * Q];
       if (a.residual) {
-        if (size == 2 && a.vec2) {
+        if (size == 2) {
 #pragma unroll
           for (int w = 0; w < W; ++w)
             res[0][w] = __builtin_amdgcn_raw_buffer_load_b32(rr, cw + uint32_t(word_row(w)) * rp, 0, 0);
-        } else if (size == 2) {
+          if (any_alone) {
 #pragma unroll
-          for (int b = 0; b < B; ++b)
-#pragma unroll
-            for (int e = 0; e < 4 * Q; ++e)
-              res[b][e] = __builtin_amdgcn_raw_buffer_load_b16(rr, cb[b] + uint32_t(row_of(e)) * rp, 0, 0);
+            for (int w = 0; w < W; ++w)
+              res[0][w] |= __builtin_amdgcn_raw_buffer_load_b16(rr, alone + uint32_t(word_row(w)) * rp, 0, 0);
+          }
         } else {
 #pragma unroll
           for (int b = 0; b < B; ++b)
@@ -415,34 +418,26 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
           for (int e = 0; e < 4 * Q; ++e) v[b][e] *= u[e];
         }
       }
-      auto store32 = [&]() {
+      if (size == 4) {
 #pragma unroll
         for (int e = 0; e < 4 * Q; ++e) {
-          float o[B];
+          if (a.residual) {
 #pragma unroll
-          for (int b = 0; b < B; ++b) o[b] = a.residual ? v[b][e] + bits_f32(res[b][e]) : v[b][e];
+            for (int b = 0; b < B; ++b) v[b][e] += bits_f32(res[b][e]);
+          }
           const uint32_t row = uint32_t(row_of(e)) * yp;
-          if (kPair && a.vec2) {
-            __builtin_amdgcn_raw_buffer_store_b64(v2u{f32_bits(o[0]), f32_bits(o[B - 1])}, yr, cb[0] + row, 0, 0);
+          if constexpr (kPair) {
+            __builtin_amdgcn_raw_buffer_store_b64(v2u{f32_bits(v[0][e]), f32_bits(v[1][e])}, yr, cw + row, 0, 0);
+            if (any_alone)
+              __builtin_amdgcn_raw_buffer_store_b32(f32_bits(v[0][e]), yr, alone + row, 0, 0);
           } else {
-#pragma unroll
-            for (int b = 0; b < B; ++b)
-              __builtin_amdgcn_raw_buffer_store_b32(f32_bits(o[b]), yr, cb[b] + row, 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b32(f32_bits(v[0][e]), yr, cb[0] + row, 0, 0);
           }
         }
-      };
+        return;
+      }
       auto store16 = [&](auto kind) {  // (the type once for all, not per value)
         constexpr int T = decltype(kind)::value;
-        if (!a.vec2) {
-#pragma unroll
-          for (int b = 0; b < B; ++b)
-#pragma unroll
-            for (int e = 0; e < 4 * Q; ++e) {
-              const float o = a.residual ? v[b][e] + from_half(res[b][e] & 0xffffu, T) : v[b][e];
-              __builtin_amdgcn_raw_buffer_store_b16(to_half(o, T), yr, cb[b] + uint32_t(row_of(e)) * yp, 0, 0);
-            }
-          return;
-        }
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           float lo, hi;
@@ -457,12 +452,12 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
             lo += from_half(res[0][w] & 0xffffu, T);
             hi += from_half(res[0][w] >> 16, T);
           }
-          __builtin_amdgcn_raw_buffer_store_b32(to_halves(lo, hi, T), yr, cw + uint32_t(word_row(w)) * yp, 0, 0);
+          const uint32_t word = to_halves(lo, hi, T), row = uint32_t(word_row(w)) * yp;
+          __builtin_amdgcn_raw_buffer_store_b32(word, yr, cw + row, 0, 0);
+          if (any_alone) __builtin_amdgcn_raw_buffer_store_b16(uint16_t(word), yr, alone + row, 0, 0);
         }
       };
-      if (a.out_type == I8CONV_FP32)
-        store32();
-      else if (a.out_type == I8CONV_BF16)
+      if (a.out_type == I8CONV_BF16)
         store16(Set<I8CONV_BF16>{});
       else
         store16(Set<I8CONV_FP16>{});

@@ -27,7 +27,7 @@ struct LinearArgs {
   int k, n, wide;          // wide = n, or 2 n where gated
   int experts;             // 0: dense
   int activation, out_type, x_type;
-  bool vec4, vec2;  // outputs may move four or two at once (linear_vec_ok)
+  bool vec4;  // few rows: four consecutive outputs may move at once (linear_vec_ok)
 };
 
 // Whether rows of n values of `size` bytes at base + row * ld may be moved

@@ -20,14 +20,14 @@ struct TileCost {
   double alone, full, besides;
 };
 const TileCost kTiles[] = {
-    {kTile256x256, 256, 256, 1, 1, 2, true, true, 1.25, 1.80, 5.0},
-    {kTile128x256, 128, 256, 1, 1, 3, true, true, 0.76, 1.10, 4.0},
-    {kTile128x128, 128, 128, 2, 1, 2, true, true, 0.66, 1.18, 3.0},
-    {kTile128x64, 128, 64, 3, 1, 2, true, true, 0.60, 1.05, 2.5},
-    {kTile64x64, 64, 64, 4, 1, 2, true, false, 0.50, 0.90, 2.0},
-    {kTile64x64Deep, 64, 64, 2, 1, 4, true, false, 0.28, 0.45, 2.0},
+    {kTile256x256, 256, 256, 1, 1, 2, true, true, 1.25, 1.80, 10.0},
+    {kTile128x256, 128, 256, 1, 1, 3, true, true, 0.76, 1.10, 6.0},
+    {kTile128x128, 128, 128, 2, 1, 2, true, true, 0.66, 1.18, 5.0},
+    {kTile128x64, 128, 64, 3, 1, 2, true, true, 0.60, 1.05, 3.5},
+    {kTile64x64, 64, 64, 4, 1, 2, true, false, 0.50, 0.90, 2.5},
+    {kTile64x64Deep, 64, 64, 2, 1, 4, true, false, 0.28, 0.45, 2.5},
     {kTile64x64Pair, 64, 64, 1, 2, 4, true, false, 0.42, 0.50, 2.5},
-    {kTile128x64Pair, 128, 64, 1, 2, 3, false, true, 0.60, 0.76, 2.5},
+    {kTile128x64Pair, 128, 64, 1, 2, 3, false, true, 0.60, 0.76, 3.0},
 };
 
 // Whole tiles and parts of one (which take about kPart of one's time) as rounds
