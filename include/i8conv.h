@@ -262,8 +262,8 @@ typedef enum i8conv_activation {
   I8CONV_ACT_SILU = 4       /* v / (1 + exp(-v)) */
 } i8conv_activation;
 
-/* A linear layer.  `rows` may be 0 (nothing is launched).  inputs % 16 == 0
- * and < 2^17; the weights of one matrix (outputs, or 2 * outputs where gated,
+/* A linear layer.  `rows` may be 0 (nothing is launched) and is below 2^29;
+ * inputs % 16 == 0 and < 2^17; the weights of one matrix (outputs, or 2 * outputs where gated,
  * times inputs) below 2^31 bytes, outputs below 2^24.  Strides are elements
  * between rows, 0 for packed rows; that of an int8 input is a multiple of 16
  * below 2^23, those of output and residual are below 2^24. */
@@ -282,6 +282,10 @@ typedef struct i8conv_linear_shape {
 /* Device memory that a launch of `shape` needs, 256-byte aligned: the codes and
  * scales of an input that is quantized on the way.  0 for a bad shape. */
 size_t i8conv_linear_workspace_bytes(const i8conv_linear_shape *shape);
+
+/* Writes which kernels a launch of `shape` runs into buf (NUL-terminated, at
+ * most len bytes), for tensors of 16-byte alignment. */
+int i8conv_linear_describe(const i8conv_linear_shape *shape, char *buf, size_t len);
 
 /* A dense layer.  `input_scale` (rows floats) belongs to an int8 input and is
  * NULL with any other, whose rows are quantized as by i8conv_quantize_rows.
@@ -312,12 +316,13 @@ int i8conv_launch_expert_linear(const i8conv_linear_shape *shape, const void *in
 /* Rows to int8 codes and their scales, with a = max |x[k]| of a row:
  *   code[k] = rint(127 x[k] / a) (half to even),  scale = a / 127.
  * A row with a < 2^-100 gives zeros and scale 0, a row with an infinity or NaN
- * zeros and scale NaN.  inputs % 16 == 0; codes are packed, 16-byte aligned. */
+ * zeros and scale NaN.  inputs % 16 == 0 and < 2^24; codes are packed, 16-byte
+ * aligned. */
 int i8conv_quantize_rows(const void *input, int type, int32_t rows, int32_t inputs,
                          int64_t input_stride, int8_t *codes, float *scales,
                          void *stream);
 
-/* tokens x choices expert ids, below 2^31 in all; at most 4096 experts. */
+/* tokens x choices expert ids, below 2^29 in all; at most 4096 experts. */
 typedef struct i8conv_route_shape {
   int32_t tokens, choices, experts;
 } i8conv_route_shape;
@@ -334,7 +339,8 @@ int i8conv_launch_route(const i8conv_route_shape *shape, const int32_t *ids,
                         int32_t *offsets, int32_t *sources, int32_t *places,
                         void *workspace, size_t workspace_bytes, void *stream);
 
-/* Packed rows of `outputs` values; neither type is INT8. */
+/* Packed rows of `outputs` (below 2^24) values, tokens x choices below 2^29;
+ * neither type is INT8. */
 typedef struct i8conv_combine_shape {
   int32_t tokens, choices, outputs;
   int32_t input_type, output_type;

@@ -45,7 +45,7 @@ __all__ = [
     "set_wait_spin_limit", "wait_spin_limit", "DEFAULT_WAIT_SPIN_LIMIT",
     "LinearShape", "RouteShape", "CombineShape", "linear_workspace_bytes", "launch_linear",
     "launch_expert_linear", "quantize_rows", "route_workspace_bytes", "launch_route",
-    "launch_combine",
+    "launch_combine", "describe_linear",
 ]
 
 KERNELS = ("generic", "strip", "halo", "splitk")
@@ -711,6 +711,13 @@ class CombineShape(_Described):
 
 def linear_workspace_bytes(shape: LinearShape) -> int:
     return int(lib().i8conv_linear_workspace_bytes(shape._c_ref()))
+
+
+def describe_linear(shape: LinearShape) -> str:
+    """The kernels a launch of `shape` runs (i8conv_linear_describe)."""
+    buf = ctypes.create_string_buffer(256)
+    check(lib().i8conv_linear_describe(shape._c_ref(), buf, 256), "describe_linear")
+    return buf.value.decode()
 
 
 def launch_linear(shape: LinearShape, input, input_scale, weight, weight_scale, bias, residual,

@@ -114,6 +114,7 @@ SIGNATURES = {
     "i8conv_unpack_vect_c": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                      c_void_p]),
     "i8conv_linear_workspace_bytes": (c_size_t, [POINTER(CLinearShape)]),
+    "i8conv_linear_describe": (c_int, [POINTER(CLinearShape), c_char_p, c_size_t]),
     "i8conv_launch_linear": (c_int, [POINTER(CLinearShape)] + [c_void_p] * 8 +
                              [c_size_t, c_void_p]),
     "i8conv_launch_expert_linear": (c_int, [POINTER(CLinearShape)] + [c_void_p] * 9 +

@@ -234,7 +234,9 @@ enum LinearTile {
   kTile64x64Pair
 };
 int launch_linear_tiles(const LinearArgs &a, bool gated, int tile, void *stream);
-// linear_policy.cpp: the tile for `rows` rows (of `experts` experts, 0: dense).
+// linear_policy.cpp: the tile for `rows` rows (of `experts` experts, 0: dense),
+// and its name (rows x weight rows).
+const char *linear_tile_name(int tile);
 int plan_linear_tile(int64_t rows, int64_t experts, int64_t n, int64_t k, bool gated);
 // kernel_linear_rows.hip: layers of few rows.  fused: a.x holds 16-byte
 // aligned values of a.x_type, a row's stride a multiple of 16 bytes, which the

@@ -2,6 +2,8 @@
 // which kernels a launch runs.
 #include <hip/hip_runtime.h>
 
+#include <stdio.h>
+
 #include <algorithm>
 #include <string>
 
@@ -12,6 +14,8 @@ namespace i8conv {
 namespace {
 
 constexpr int kMaxExperts = 4096;
+constexpr int kMaxRows = 1 << 29;            // their scales are addressed with 31 bits
+constexpr int64_t kMaxOutputs = int64_t(1) << 40;  // rows x weight rows: tile numbers fit an int
 constexpr int64_t kMaxBytes = (int64_t(1) << 31) - 1;
 
 bool aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
@@ -28,6 +32,9 @@ int check_shape(const i8conv_linear_shape *s) {
   if (!s) return fail(I8CONV_BAD_ARGUMENT, "null shape");
   if (s->rows < 0 || s->outputs < 1 || s->experts < 0 || s->routed < 0 || s->experts > kMaxExperts)
     return fail(I8CONV_BAD_SHAPE, "linear: rows, routed >= 0, outputs >= 1 and 0 <= experts <= 4096");
+  if (s->rows >= kMaxRows || s->routed >= kMaxRows ||
+      (int64_t(std::max(s->rows, s->routed)) * s->outputs) << 1 >= kMaxOutputs)
+    return fail(I8CONV_BAD_SHAPE, "linear: rows must be below 2^29, and rows x outputs below 2^39");
   if (s->inputs < 16 || s->inputs % 16 != 0 || s->inputs >= 1 << 17)
     return fail(I8CONV_BAD_SHAPE, "linear: inputs must be a multiple of 16 below 2^17");
   if (s->input_type != I8CONV_INT8 && !float_type(s->input_type))
@@ -163,9 +170,9 @@ int run(const i8conv_linear_shape &s, const void *input, const float *input_scal
 int check_route(const i8conv_route_shape *s) {
   if (!s) return fail(I8CONV_BAD_ARGUMENT, "null shape");
   if (s->tokens < 0 || s->choices < 1 || s->experts < 1 || s->experts > kMaxExperts ||
-      int64_t(s->tokens) * s->choices > kMaxBytes)
+      int64_t(s->tokens) * s->choices >= kMaxRows)
     return fail(I8CONV_BAD_SHAPE,
-                "route: tokens >= 0, choices >= 1, 1 <= experts <= 4096 and tokens * choices < 2^31");
+                "route: tokens >= 0, choices >= 1, 1 <= experts <= 4096 and tokens * choices < 2^29");
   return I8CONV_OK;
 }
 
@@ -178,6 +185,24 @@ extern "C" {
 
 size_t i8conv_linear_workspace_bytes(const i8conv_linear_shape *shape) {
   return check_shape(shape) == I8CONV_OK ? workspace_bytes(*shape) : 0;
+}
+
+int i8conv_linear_describe(const i8conv_linear_shape *shape, char *buf, size_t len) {
+  const int rc = check_shape(shape);
+  if (rc != I8CONV_OK) return rc;
+  if (!buf || len == 0) return fail(I8CONV_BAD_ARGUMENT, "linear: no buffer to describe into");
+  const i8conv_linear_shape &s = *shape;
+  // (as for tensors of 16-byte alignment)
+  const RowsPlan plan = plan_rows(s, nullptr);
+  const char *const first = s.input_type == I8CONV_INT8 || plan.fused ? "" : "quantize rows, ";
+  if (plan.few) {
+    snprintf(buf, len, "%sfew rows%s", first, plan.fused ? ", quantized by the workgroups" : "");
+    return I8CONV_OK;
+  }
+  const int tile = plan_linear_tile(s.experts ? s.routed : s.rows, s.experts, s.outputs, s.inputs,
+                                    s.gated != 0);
+  snprintf(buf, len, "%stiles of %s", first, linear_tile_name(tile));
+  return I8CONV_OK;
 }
 
 int i8conv_launch_linear(const i8conv_linear_shape *shape, const void *input,
@@ -223,10 +248,10 @@ int i8conv_launch_expert_linear(const i8conv_linear_shape *shape, const void *in
 int i8conv_quantize_rows(const void *input, int type, int32_t rows, int32_t inputs,
                          int64_t input_stride, int8_t *codes, float *scales, void *stream) {
   if (!float_type(type) || rows < 0 || inputs < 16 || inputs % 16 != 0 ||
-      (input_stride != 0 && input_stride < inputs))
+      inputs >= kLinearMaxStride || (input_stride != 0 && input_stride < inputs))
     return fail(I8CONV_BAD_ARGUMENT,
-                "quantize_rows: a floating type, rows >= 0, inputs a positive multiple of 16 and a "
-                "stride of 0 or at least inputs");
+                "quantize_rows: a floating type, rows >= 0, inputs a positive multiple of 16 below "
+                "2^24 and a stride of 0 or at least inputs");
   if (rows == 0) return I8CONV_OK;
   if (!input || !codes || !scales)
     return fail(I8CONV_BAD_ARGUMENT, "quantize_rows: null tensor pointer");
@@ -265,9 +290,9 @@ int i8conv_launch_combine(const i8conv_combine_shape *shape, const void *input,
                           void *output, void *stream) {
   if (!shape) return fail(I8CONV_BAD_ARGUMENT, "null shape");
   if (shape->tokens < 0 || shape->choices < 1 || shape->outputs < 1 ||
-      int64_t(shape->tokens) * shape->choices > kMaxBytes)
+      shape->outputs >= kLinearMaxStride || int64_t(shape->tokens) * shape->choices >= kMaxRows)
     return fail(I8CONV_BAD_SHAPE,
-                "combine: tokens >= 0, choices >= 1, outputs >= 1 and tokens * choices < 2^31");
+                "combine: tokens >= 0, choices >= 1, 1 <= outputs < 2^24 and tokens * choices < 2^29");
   if (!float_type(shape->input_type) || !float_type(shape->output_type))
     return fail(I8CONV_BAD_SHAPE, "combine: types are bf16, fp16 or fp32");
   if (shape->tokens == 0) return I8CONV_OK;

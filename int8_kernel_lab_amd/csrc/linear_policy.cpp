@@ -46,6 +46,20 @@ double cost(const TileCost &t, double row_tiles, int64_t wide, int64_t k) {
 
 }  // namespace
 
+const char *linear_tile_name(int tile) {
+  switch (tile) {
+    case kTile256x256: return "256 rows x 256";
+    case kTile128x256: return "128 rows x 256";
+    case kTile128x128: return "128 rows x 128";
+    case kTile128x64: return "128 rows x 64";
+    case kTile128x64Pair: return "128 rows x 64, two groups of waves";
+    case kTile64x64: return "64 rows x 64";
+    case kTile64x64Deep: return "64 rows x 64, four stages";
+    case kTile64x64Pair: return "64 rows x 64, two groups of waves";
+  }
+  return "?";
+}
+
 int plan_linear_tile(int64_t rows, int64_t experts, int64_t n, int64_t k, bool gated) {
   int best = kTile128x128;
   double least = 1e300;

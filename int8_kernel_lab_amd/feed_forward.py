@@ -1,0 +1,168 @@
+"""A feed-forward layer of a language model on the int8 linear operators.
+
+    python -m int8_kernel_lab_amd.feed_forward --tokens 64 --experts 16 --choices 4
+
+runs, on seeded fp16 activations and int8 weights, with --experts 0 the dense layer
+
+    y = x + W2 (silu(W1a x) * (W1b x))
+
+(two launch_linear calls, the second with the residual), else the same layer of
+experts (launch_route, two launch_expert_linear calls, launch_combine), checks
+the result against numpy in 64 bits and prints one JSON line with the kernels of
+each product and the time of a pass.  No counterpart in the reference.
+"""
+from __future__ import annotations
+
+import argparse
+import json
+import time
+from typing import Dict, Optional
+
+import numpy as np
+
+import int8_kernel_lab_amd as lab
+
+
+class FeedForward:
+    """The layer's weights and workspaces on the GPU, and one pass over them."""
+
+    def __init__(self, tokens: int, width: int, hidden: int, experts: int = 0, choices: int = 0,
+                 seed: int = lab.BASELINE_SEED):
+        self.tokens, self.width, self.hidden = tokens, width, hidden
+        self.experts, self.choices = experts, choices
+        rng = np.random.default_rng(seed)
+        sets = max(1, experts)
+        routed = tokens * choices
+        self.host = {
+            "x": rng.standard_normal((tokens, width)).astype(np.float16),
+            "w1": np.clip(np.rint(33 * rng.standard_normal((sets, 2 * hidden, width))), -127,
+                          127).astype(np.int8),
+            "w2": np.clip(np.rint(33 * rng.standard_normal((sets, width, hidden))), -127,
+                          127).astype(np.int8),
+            "s1": (1 / (33 * np.sqrt(width)) * np.ones((sets, 2 * hidden))).astype(np.float32),
+            "s2": (1 / (33 * np.sqrt(hidden)) * np.ones((sets, width))).astype(np.float32),
+        }
+        if experts:
+            ids = np.argsort(rng.random((tokens, experts)), axis=1)[:, :choices]
+            weights = rng.random((tokens, choices)) + 0.1
+            self.host["ids"] = np.ascontiguousarray(ids, dtype=np.int32)
+            self.host["weights"] = (weights / weights.sum(1, keepdims=True)).astype(np.float32)
+            self.up = lab.LinearShape(tokens, width, hidden, "fp16", "fp16", "silu", gated=True,
+                                      experts=experts, routed=routed)
+            self.down = lab.LinearShape(routed, hidden, width, "fp16", "fp16", experts=experts,
+                                        routed=routed)
+            self.route = lab.RouteShape(tokens, choices, experts)
+            self.sum = lab.CombineShape(tokens, choices, width, "fp16", "fp16")
+        else:
+            self.up = lab.LinearShape(tokens, width, hidden, "fp16", "fp16", "silu", gated=True)
+            self.down = lab.LinearShape(tokens, hidden, width, "fp16", "fp16")
+        self.buf: Dict[str, lab.DeviceBuffer] = {
+            name: lab.DeviceBuffer.from_array(a) for name, a in self.host.items()}
+        rows = routed if experts else tokens
+        self.buf["h"] = lab.DeviceBuffer(2 * rows * hidden)
+        self.buf["y"] = lab.DeviceBuffer(2 * tokens * width)
+        need = max(lab.linear_workspace_bytes(self.up), lab.linear_workspace_bytes(self.down))
+        if experts:
+            self.buf["z"] = lab.DeviceBuffer(2 * routed * width)
+            self.buf["offsets"] = lab.DeviceBuffer(4 * (experts + 1))
+            self.buf["sources"] = lab.DeviceBuffer(4 * routed)
+            self.buf["places"] = lab.DeviceBuffer(4 * routed)
+            need = max(need, lab.route_workspace_bytes(self.route))
+        self.buf["workspace"] = lab.DeviceBuffer(max(1, need))
+
+    def launch(self, stream: Optional[int] = None) -> None:
+        """One pass, asynchronous."""
+        b = self.buf
+        if not self.experts:
+            lab.launch_linear(self.up, b["x"], None, b["w1"], b["s1"], None, None, b["h"],
+                              b["workspace"], stream=stream)
+            lab.launch_linear(self.down, b["h"], None, b["w2"], b["s2"], None, b["x"], b["y"],
+                              b["workspace"], stream=stream)
+            return
+        lab.launch_route(self.route, b["ids"], b["offsets"], b["sources"], b["places"],
+                         b["workspace"], stream=stream)
+        lab.launch_expert_linear(self.up, b["x"], None, b["w1"], b["s1"], None, b["offsets"],
+                                 b["sources"], b["h"], b["workspace"], stream=stream)
+        lab.launch_expert_linear(self.down, b["h"], None, b["w2"], b["s2"], None, b["offsets"], None,
+                                 b["z"], b["workspace"], stream=stream)
+        lab.launch_combine(self.sum, b["z"], b["places"], b["weights"], b["x"], b["y"],
+                           stream=stream)
+
+    def output(self) -> np.ndarray:
+        """What the last pass wrote (synchronizes)."""
+        lab.synchronize()
+        return self.buf["y"].download(np.float16, self.tokens * self.width).reshape(
+            self.tokens, self.width)
+
+    def describe(self) -> str:
+        return f"up: {lab.describe_linear(self.up)}; down: {lab.describe_linear(self.down)}"
+
+    def close(self) -> None:
+        for b in self.buf.values():
+            b.close()
+
+
+def quantize(x: np.ndarray):
+    """Codes and row scales in 64 bits."""
+    x = x.astype(np.float64)
+    top = np.abs(x).max(axis=1, keepdims=True)
+    top[top < 2.0 ** -100] = np.inf
+    return np.rint(127 * x / top), np.where(np.isinf(top), 0.0, top / 127)
+
+
+def expected(layer: FeedForward) -> np.ndarray:
+    """The layer's output in numpy, 64 bits but for the rounding of the hidden
+    values to fp16, which the layer stores."""
+    h = layer.host
+    codes, scale = quantize(h["x"])
+    out = h["x"].astype(np.float64)
+    for e in range(max(1, layer.experts)):
+        if layer.experts:
+            token, choice = np.nonzero(h["ids"] == e)
+            weight = h["weights"][token, choice].astype(np.float64)[:, None]
+        else:
+            token, weight = np.arange(layer.tokens), 1.0
+        if token.size == 0:
+            continue
+        v = codes[token] @ h["w1"][e].T.astype(np.float64) * scale[token] * h["s1"][e]
+        a, u = v[:, :layer.hidden], v[:, layer.hidden:]
+        hidden, hs = quantize((a / (1 + np.exp(-a)) * u).astype(np.float16))
+        z = hidden @ h["w2"][e].T.astype(np.float64) * hs * h["s2"][e]
+        np.add.at(out, token, weight * z)
+    return out
+
+
+def main(argv=None) -> int:
+    ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
+    ap.add_argument("--tokens", type=int, default=16)
+    ap.add_argument("--width", type=int, default=1024)
+    ap.add_argument("--hidden", type=int, default=2048)
+    ap.add_argument("--experts", type=int, default=8, help="0: a dense layer")
+    ap.add_argument("--choices", type=int, default=2)
+    ap.add_argument("--iterations", type=int, default=100)
+    a = ap.parse_args(argv)
+    layer = FeedForward(a.tokens, a.width, a.hidden, a.experts, a.choices if a.experts else 0)
+    try:
+        layer.launch()
+        got, want = layer.output().astype(np.float64), expected(layer)
+        # hidden values, expert rows and output are each rounded to fp16, by at
+        # most 2^-11 of a value, and a rounded hidden value can move its code
+        # by one: below 4 x 2^-11 of the output's norm
+        error = float(np.linalg.norm(got - want) / np.linalg.norm(want))
+        lab.synchronize()
+        began = time.perf_counter()
+        for _ in range(a.iterations):
+            layer.launch()
+        lab.synchronize()
+        us = (time.perf_counter() - began) / max(1, a.iterations) * 1e6
+        print(json.dumps({"layer": "experts" if a.experts else "dense", "tokens": a.tokens,
+                          "width": a.width, "hidden": a.hidden, "experts": a.experts,
+                          "choices": layer.choices, "kernels": layer.describe(),
+                          "relative_error": error, "us_per_pass": us}), flush=True)
+        return 0 if error < 4 * 2.0 ** -11 else 1
+    finally:
+        layer.close()
+
+
+if __name__ == "__main__":
+    raise SystemExit(main())

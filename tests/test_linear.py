@@ -505,6 +505,35 @@ def test_experts_of_most_experts():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("counts", [[4] * 4096, [e % 9 for e in range(2050)]], ids=["4096", "2050"])
+def test_experts_of_many_experts_in_tiles(counts):
+    run_experts(counts, 32, 24, tokens=100, y="fp32")
+    run_experts(counts, 32, 24, tokens=100, gated=True, bias=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("odd", [1, 3, 63, 65, 129, 255])
+@pytest.mark.parametrize("rows", [40, 500, 3000])
+def test_linear_last_channel_alone(odd, rows):
+    # odd channel counts in every tile: the last one leaves by itself
+    for y in ("bf16", "fp32"):
+        run_linear(rows, 144, odd, y=y, residual=True, strides=(0, odd + 2, odd + 4))
+        run_linear(rows, 144, odd, y=y, residual=True, gated=True, offset=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("experts,choices", [(0, 0), (8, 2)])
+@pytest.mark.parametrize("tokens", [1, 37])
+def test_feed_forward_example(experts, choices, tokens, capsys):
+    from int8_kernel_lab_amd import feed_forward
+    say(f"[gpu] feed forward, {tokens} tokens, {experts} experts")
+    assert feed_forward.main(["--tokens", str(tokens), "--width", "256", "--hidden", "400",
+                              "--experts", str(experts), "--choices", str(max(1, choices)),
+                              "--iterations", "2"]) == 0
+    assert '"relative_error"' in capsys.readouterr().out
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [4, 90])
 def test_experts_sources_outside_read_as_zeros(rows):
     say(f"[gpu] sources outside, {rows} rows")
@@ -698,3 +727,63 @@ def test_bad_route_and_combine_arguments_are_refused():
         tensors = [FAKE] * 5
         tensors[i] = spoilt
         assert combine(good, *tensors) == _lib.BAD_ARGUMENT, i
+
+
+def test_sizes_beyond_the_limits_are_refused():
+    for shape, reason in ((lab.LinearShape(1 << 29, 64, 32), "2^29"),
+                          (lab.LinearShape(1 << 24, 16, 1 << 15), "2^39"),
+                          (lab.LinearShape(4, 16, 1 << 24), "2^24"),
+                          (lab.LinearShape(4, 64, 32, output_stride=1 << 24), "2^24")):
+        assert _linear_rc(shape) == _lib.BAD_SHAPE
+        assert reason in _lib.lib().i8conv_last_error().decode()
+    wide = lab.CombineShape(4, 2, 1 << 24).c_struct()
+    assert _lib.lib().i8conv_launch_combine(ctypes.byref(wide), *[FAKE] * 5, None) == _lib.BAD_SHAPE
+    assert _lib.lib().i8conv_quantize_rows(FAKE, 1, 4, 1 << 24, 0, FAKE, FAKE, None) == _lib.BAD_ARGUMENT
+
+
+def test_route_workspace_is_asked_for():
+    shape = lab.RouteShape(40000, 8, 128)
+    need = lab.route_workspace_bytes(shape)
+    assert need > 0 and lab.route_workspace_bytes(lab.RouteShape(8, 8, 128)) == 0
+    for workspace, nbytes in ((None, need), (FAKE, need - 1), (FAKE + 128, need)):
+        rc = _lib.lib().i8conv_launch_route(ctypes.byref(shape.c_struct()), FAKE, FAKE, FAKE, FAKE,
+                                            workspace, nbytes, None)
+        assert rc == _lib.WORKSPACE_TOO_SMALL
+        assert str(need) in _lib.lib().i8conv_last_error().decode()
+
+
+def test_linear_plans_are_described():
+    assert "few rows" in lab.describe_linear(lab.LinearShape(1, 4096, 4096))
+    assert "quantize rows" not in lab.describe_linear(lab.LinearShape(500, 4096, 4096, "int8"))
+    assert lab.describe_linear(lab.LinearShape(16384, 8192, 8192)).endswith("256 rows x 256")
+    for rows in (33, 200, 1000, 5000):
+        for gated in (False, True):
+            for experts in (0, 64, 4096):
+                shape = lab.LinearShape(rows, 1024, 1000, gated=gated, experts=experts,
+                                        routed=rows * 4 if experts else 0)
+                assert "?" not in lab.describe_linear(shape)
+    with pytest.raises(lab.I8ConvError):
+        lab.describe_linear(lab.LinearShape(4, 24, 8))
+    buf = ctypes.create_string_buffer(4)
+    c = lab.LinearShape(1, 64, 64).c_struct()
+    assert _lib.lib().i8conv_linear_describe(ctypes.byref(c), buf, 4) == _lib.OK
+    assert len(buf.value) == 3  # cut, and ended
+    assert _lib.lib().i8conv_linear_describe(ctypes.byref(c), None, 4) == _lib.BAD_ARGUMENT
+
+
+def test_linear_shapes_are_values():
+    import pickle
+    shape = lab.LinearShape(7, 64, 33, experts=4, routed=14)
+    shape._c_ref()
+    assert pickle.loads(pickle.dumps(shape)) == shape
+    assert (shape.weight_rows, shape.ops()) == (33, 2 * 14 * 33 * 64)
+    assert lab.LinearShape(7, 64, 33, gated=True).weight_rows == 66
+
+
+def test_feed_forward_reference_is_the_formula():
+    # the example's own numbers on the CPU: one token, one expert, by hand
+    from int8_kernel_lab_amd import feed_forward
+    import numpy as np
+    codes, scale = feed_forward.quantize(np.array([[0.5, -1.0, 0.25, 0.0], [0, 0, 0, 0]]))
+    assert codes.tolist() == [[64, -127, 32, 0], [0, 0, 0, 0]]  # 63.5 to even
+    assert scale[1, 0] == 0 and scale[0, 0] == 1 / 127
