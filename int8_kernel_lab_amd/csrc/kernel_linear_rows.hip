@@ -31,8 +31,16 @@ namespace {
 constexpr int kRowsWaves = 8, kRowsThreads = 64 * kRowsWaves;
 // 8-value pieces of x a thread holds: 16 registers of 16-bit or 32-bit values.
 constexpr int fused_chunks(int size) { return size == 4 ? 2 : 4; }
-constexpr int kFusedLds = 256;  // bytes of their largest values and the rows' scales
-static_assert(fused_chunks(2) * (kRowsWaves + 1) * 4 <= kFusedLds, "fits");
+constexpr int kFusedLds = fused_chunks(2) * kRowsWaves * 4;  // bytes of their largest values
+
+// What a workgroup's sums meet at the end: per channel (the second half of
+// gated ones last) weight scales and biases, the residual of rows and channels,
+// the rows' scales.  A thread reads at most one value of each kind, at the
+// beginning: read where they are needed, they cost a memory's latency.
+template <int F, int C, int MF>
+struct alignas(16) RowsLast {
+  float scale[16 * F], bias[16 * F], residual[16 * MF][16 * C], row_scale[16 * MF];
+};
 
 // Bytes between rows of codes in LDS: 16-byte units in a step of 2 x odd, so
 // that a fragment read (16 rows, two chunks per 32 lanes) has no bank conflicts.
@@ -76,17 +84,21 @@ __global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearA
   constexpr int F = kGated ? 2 * C : C;
   constexpr bool kFused = kX != 0;
   constexpr int kChunks = fused_chunks(kX);
-  // LDS: the waves' sums; kFused: the pieces' largest values, the rows' scales
-  // and their codes [step_rows][pitch]
+  // LDS: the waves' sums; what the last step needs besides; kFused: the pieces'
+  // largest values and the rows' codes [step_rows][pitch]
   extern __shared__ __attribute__((aligned(16))) int8_t smem[];
   v4i(*const sums)[F * MF][64] = reinterpret_cast<v4i(*)[F * MF][64]>(smem);
-  int8_t *const extra = smem + sizeof(v4i) * kRowsWaves * F * MF * 64;
-  uint32_t(*const tops)[kRowsWaves] = reinterpret_cast<uint32_t(*)[kRowsWaves]>(extra);
-  float *const row_scale = reinterpret_cast<float *>(extra + kChunks * kRowsWaves * 4);
-  int8_t *const codes = extra + kFusedLds;
+  RowsLast<F, C, MF> *const last =
+      reinterpret_cast<RowsLast<F, C, MF> *>(smem + sizeof(v4i) * kRowsWaves * F * MF * 64);
+  uint32_t(*const tops)[kRowsWaves] = reinterpret_cast<uint32_t(*)[kRowsWaves]>(last + 1);
+  int8_t *const codes = reinterpret_cast<int8_t *>(last + 1) + kFusedLds;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool gather = kExperts && a.sources != nullptr;
+  // (the first of them, without waiting for the group)
+  const int first_source =
+      kFused && kExperts && a.sources && lane < a.rows ? a.sources[lane] : -1;
   Group group = {0, 0, a.rows};
   if constexpr (kExperts) {
     if (!find_group(a.offsets, a.experts, a.rows, int(blockIdx.y), lane, &group)) return;
@@ -94,7 +106,6 @@ __global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearA
     group.begin = __builtin_amdgcn_readfirstlane(group.begin);
     group.end = __builtin_amdgcn_readfirstlane(group.end);
   }
-  const bool gather = kExperts && a.sources != nullptr;
   const int q = lane & 15, kq = 16 * (lane >> 4);
   const int c0 = int(blockIdx.x) * 16 * C;
 
@@ -119,6 +130,15 @@ __global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearA
       }
   };
 
+  // this thread's weight scale or bias
+  float param = 0.0f;
+  {
+    const int f = int(threadIdx.x) % (16 * F) / 16, ch = c0 + 16 * (f % C) + int(threadIdx.x) % 16;
+    const float *const from = threadIdx.x < 16 * F ? a.ws : a.bias;
+    if (threadIdx.x < 32 * F && from && ch < a.n)
+      param = from[int64_t(group.expert) * a.wide + ch + (f >= C ? a.n : 0)];
+  }
+
   const int pitch = fused_pitch(a.k);
   // rows of x per pass
   const int chunks = (a.k + 8 * kRowsThreads - 1) / (8 * kRowsThreads);
@@ -126,8 +146,16 @@ __global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearA
   for (int row0 = group.begin; row0 < group.end; row0 += step_rows) {
     const int rows = min(step_rows, group.end - row0);
 
+    // this thread's value of the residual
+    float res = 0.0f, xs_of = 0.0f;
+    {
+      const int r = int(threadIdx.x) / (16 * C), ch = c0 + int(threadIdx.x) % (16 * C);
+      if (a.residual && r < min(rows, 16 * MF) && ch < a.n)
+        res = load_value(a.residual, int64_t(row0 + r) * a.ldr + ch, a.out_type);
+    }
+
     // codes: this lane's row of each fragment
-    uint32_t xoff[MF];
+    uint32_t src[MF], xoff[MF];
     const int8_t *const xbase =
         static_cast<const int8_t *>(a.x) + (gather || kFused ? 0 : int64_t(row0) * a.ldx);
     const auto xr = make_rsrc(xbase, kFused ? 0u
@@ -136,13 +164,9 @@ __global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearA
     if constexpr (!kFused) {
 #pragma unroll
       for (int m = 0; m < MF; ++m) {
-        uint32_t r = uint32_t(16 * m + q);
-        bool ok = int(r) < rows;
-        if (gather && ok) {
-          r = uint32_t(a.sources[row0 + int(r)]);
-          ok = r < uint32_t(a.x_rows);
-        }
-        xoff[m] = ok ? r * uint32_t(a.ldx) + uint32_t(kq) : kOutOfRange;
+        const int r = 16 * m + q;
+        src[m] = r < rows ? uint32_t(r) : kOutOfRange;
+        if (gather && r < rows) src[m] = uint32_t(a.sources[row0 + r]);
       }
     }
 
@@ -165,9 +189,9 @@ __global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearA
           if (c == chunks) c = 0, ++r;
           const int k = piece + c * 8 * kRowsThreads;
           int64_t src = row0 + r;
-          bool ok = r < rows && k < a.k;
-          if (gather && ok) src = a.sources[src];
-          ok = ok && uint64_t(src) < uint64_t(a.x_rows);
+          if (gather && r < rows)
+            src = src < 64 ? __builtin_amdgcn_readlane(first_source, int(src)) : a.sources[src];
+          const bool ok = r < rows && k < a.k && uint64_t(src) < uint64_t(a.x_rows);
           const int8_t *const p = static_cast<const int8_t *>(a.x) + (src * a.ldx + k) * kX;
 #pragma unroll
           for (int w = 0; w < kWords; w += 4) {
@@ -206,7 +230,7 @@ __global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearA
 #pragma unroll
           for (int w = 0; w < kRowsWaves; ++w) top = max(top, tops[r * chunks + j][w]);
         const RowStep step = row_step(top);
-        if (threadIdx.x == 0) row_scale[r] = step.scale;
+        if (threadIdx.x == 0) last->row_scale[r] = step.scale;
         float t[8];
         piece_of(i, t);
         if (k < a.k) *reinterpret_cast<v2u *>(codes + r * pitch + k) = codes8(t, step);
@@ -214,6 +238,13 @@ __global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearA
       __syncthreads();
     } else {
       load_w(wv, k0);
+#pragma unroll
+      for (int m = 0; m < MF; ++m) {
+        // (of dense rows src is the row within the step)
+        const bool ok = gather ? src[m] < uint32_t(a.x_rows) : src[m] != kOutOfRange;
+        xoff[m] = ok ? src[m] * uint32_t(a.ldx) + uint32_t(kq) : kOutOfRange;
+        if (ok && int(threadIdx.x) == 16 * m + q) xs_of = a.xs[gather ? src[m] : uint32_t(row0) + src[m]];
+      }
     }
 #pragma unroll 1
     for (int k = k0; k < k1; k += 64 * U) {
@@ -243,6 +274,13 @@ __global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearA
     for (int f = 0; f < F; ++f)
 #pragma unroll
       for (int m = 0; m < MF; ++m) sums[wave][f * MF + m][lane] = acc[f][m];
+    if (threadIdx.x < 16 * F)
+      last->scale[threadIdx.x] = param;
+    else if (threadIdx.x < 32 * F)
+      last->bias[threadIdx.x - 16 * F] = param;
+    if (threadIdx.x < 256 * MF * C)
+      last->residual[threadIdx.x / (16 * C)][threadIdx.x % (16 * C)] = res;
+    if (!kFused && threadIdx.x < 16 * MF) last->row_scale[threadIdx.x] = xs_of;
     __syncthreads();
     // each wave finishes 16 channels of 16 rows
     for (int part = wave; part < C * MF; part += kRowsWaves) {
@@ -257,41 +295,32 @@ __global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearA
         for (int w = 1; w < kRowsWaves; ++w) s[h] += sums[w][f][lane];
       }
       if (r < rows && ch < a.n) {
-        float xs;
-        if constexpr (kFused) {
-          xs = row_scale[r];
-        } else {
-          const int src = gather ? a.sources[row0 + r] : row0 + r;
-          xs = uint32_t(src) < uint32_t(a.x_rows) ? a.xs[src] : 0.0f;
-        }
+        const float xs = last->row_scale[r];
         float v[4], u[4];
-        const int64_t p = int64_t(group.expert) * a.wide + ch;
+        const int p = 16 * c + 4 * (lane >> 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool ok = ch + e < a.n;
-          v[e] = fmaf(float(s[0][e]) * xs, ok ? a.ws[p + e] : 0.0f, ok && a.bias ? a.bias[p + e] : 0.0f);
+          v[e] = fmaf(float(s[0][e]) * xs, last->scale[p + e], last->bias[p + e]);
           if constexpr (kGated)
-            u[e] = fmaf(float(s[kGated][e]) * xs, ok ? a.ws[p + a.n + e] : 0.0f,
-                        ok && a.bias ? a.bias[p + a.n + e] : 0.0f);
+            u[e] = fmaf(float(s[kGated][e]) * xs, last->scale[16 * C + p + e],
+                        last->bias[16 * C + p + e]);
         }
         activate(v, a.activation);
         if constexpr (kGated) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] *= u[e];
         }
-        const int64_t row = row0 + r;
+        const int64_t at = int64_t(row0 + r) * a.ldy + ch;
+        if (a.residual) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] += last->residual[r][p + e];
+        }
         if (a.vec4) {
-          v4f o = {v[0], v[1], v[2], v[3]};
-          if (a.residual) o += load_values4(a.residual, row * a.ldr + ch, a.out_type);
-          store_values4(a.y, row * a.ldy + ch, a.out_type, o);
+          store_values4(a.y, at, a.out_type, v4f{v[0], v[1], v[2], v[3]});
         } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (ch + e >= a.n) break;
-            float o = v[e];
-            if (a.residual) o += load_value(a.residual, row * a.ldr + ch + e, a.out_type);
-            store_value(a.y, row * a.ldy + ch + e, a.out_type, o);
-          }
+          for (int e = 0; e < 4; ++e)
+            if (ch + e < a.n) store_value(a.y, at + e, a.out_type, v[e]);
         }
       }
     }
@@ -302,7 +331,10 @@ __global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearA
 template <bool kGated, bool kExperts, int kX, int C, int MF, int U, int kOcc>
 int launch_rows(const LinearArgs &a, hipStream_t s) {
   auto kern = linear_rows_kernel<kGated, kExperts, kX, C, MF, U, kOcc>;
-  const size_t lds = size_t(kRowsWaves) * (kGated ? 2 : 1) * C * MF * 1024 +
+  constexpr int F = (kGated ? 2 : 1) * C;
+  static_assert(32 * F <= kRowsThreads && 256 * MF * C <= kRowsThreads && fused_chunks(2) <= 16,
+                "a value of each kind per thread");
+  const size_t lds = size_t(kRowsWaves) * F * MF * 1024 + sizeof(RowsLast<F, C, MF>) +
                      (kX ? kFusedLds + size_t(fused_rows(a.k, kX)) * fused_pitch(a.k) : 0);
   static LdsLimit limit;
   if (const int rc = limit.raise(kern, lds); rc != I8CONV_OK) return rc;
