@@ -127,9 +127,10 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
   }
   const TileRun run = xcd_tile_run(tiles_m * tiles_n, int(gridDim.x), int(blockIdx.x));
 
-  // copies: this lane's row within a copy's eight and its chunk of the row
-  const int crow = lane / (P / 16);
-  const int lk = 16 * ((lane % (P / 16)) ^ swz32_f(wave * RPC + crow));
+  // copies: the lane, its row within a copy's eight and its chunk of the row;
+  // anew for each tile (kept across the sums, what the first copies need was
+  // spilled, and each reload waited for the copies before it)
+  int clane = 0, crow = 0, lk = 0;
   // fragment reads: row lane % 32, chunk 2 ks + lane / 32
   const int frow = lane & 31, ff = swz32_f(frow);
   int koff[KS];
@@ -147,6 +148,10 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
   // inside the tensors: their sums go nowhere.  Chunks past k have to be zero
   // in one operand, and are in x.
   auto setup = [&](int t) {
+    clane = lane;
+    asm volatile("" : "+v"(clane));
+    crow = clane / (P / 16);
+    lk = 16 * ((clane % (P / 16)) ^ swz32_f(wave * RPC + crow));
     const int in_group = kRowGroup * tiles_n, g = t / in_group, m0 = g * kRowGroup;
     const int gm = min(kRowGroup, tiles_m - m0), at = t - g * in_group;
     const int tm = m0 + at % gm;
@@ -215,13 +220,13 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
     const v4u rd = make_desc(a.xs, uint32_t(a.x_rows) * 4u);
     for (int i0 = wave_id * 64; i0 < BN + BM; i0 += 64 * kWaves * KG) {
       if (i0 < BN) {
-        const int c = i0 + lane, half = kGated && c >= BO;
+        const int c = i0 + clane, half = kGated && c >= BO;
         const int ch = n0 + c - (half ? BO : 0);
         const uint32_t off = ch < a.n ? uint32_t(ch + (half ? a.n : 0)) * 4u : kOutOfRange;
         lds_copy4(sd, dst + uint32_t(i0) * 4u, off);
         lds_copy4(bd, dst + uint32_t(BN + i0) * 4u, off);
       } else {
-        const int m = i0 - BN + lane;
+        const int m = i0 - BN + clane;
         uint32_t r = uint32_t(row0 + m);
         if (m < rows && gather) r = uint32_t(a.sources[row0 + m]);
         lds_copy4(rd, dst + uint32_t(BN + i0) * 4u, m < rows && r < uint32_t(a.x_rows) ? r * 4u : kOutOfRange);
@@ -337,81 +342,119 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
     t += run.step;
     const bool again = t < run.last;
 
-    // Outputs of rows 8 g + 4 (lane / 32) + e of the wave's output block i (kPair:
-    // of i and i + 1), row block j, from the lane's sums of quad g (all in 32 bits)
+    // The outputs leave in steps of Q quads (rows 8 g + 4 (lane / 32) + e of a row
+    // block, g0 <= g < g0 + Q) of B of the wave's output blocks, in 32 bits until
+    // the last rounding.
     constexpr int B = kPair ? 2 : 1;
-    const int half = lane >> 5;
-    // Q quads, from g0 on, of row block j: their sums sg (and su, the other
-    // halves'), for each of the B blocks
     constexpr int Q = kGated || kOcc == 3 ? 1 : 2;  // (two spill there)
-    auto finish = [&](int i, int j, int g0, const v4i (&sg)[B][Q], const v4i (&su)[B][Q]) {
-      const int ct = wn * (32 * FO) + (kPair ? i * 32 + 2 * (lane & 31) : 32 * i + (lane & 31));
-      const int ch = out_n + ct;
-      const int r0 = wm * TM + 32 * j + 4 * half + 8 * g0;
-      // windows over this step's rows, its first one at 0: rows past the tile's
-      // last are out of their range, and so is the column of a channel past n
-      const int size = a.out_type == I8CONV_FP32 ? 4 : 2;
-      const int w0 = wm * TM + 32 * j + 8 * g0, left = out_rows - w0;
-      const uint32_t yp = uint32_t(a.ldy) * uint32_t(size), rp = uint32_t(a.ldr) * uint32_t(size);
-      const auto window = [&](const void *base, int64_t ld, uint32_t pitch) {
-        const int in = min(left, 8 * Q);
-        return make_rsrc(static_cast<const int8_t *>(base) + (out_row + w0) * ld * size,
-                         in > 0 && base ? uint32_t(in - 1) * pitch + uint32_t(a.n) * uint32_t(size) : 0u);
-      };
-      const auto yr = window(a.y, a.ldy, yp), rr = window(a.residual, a.ldr, rp);
-      auto row_of = [&](int e) { return 4 * half + 8 * (e / 4) + e % 4; };
-      // 16-bit outputs leave two channels to a dword, at any alignment (buffer
-      // accesses need none).  Single blocks: of every two rows an even lane takes
-      // the first and its odd neighbour the second.  With n odd the last channel
-      // is alone.
-      const int odd = kPair ? 0 : lane & 1, pair = ch - odd;
-      constexpr int W = kPair ? 4 * Q : 2 * Q;  // dwords
-      auto word_row = [&](int w) { return kPair ? row_of(w) : row_of(2 * w) + odd; };
-      const uint32_t cw = pair + 1 < a.n ? uint32_t(pair) * uint32_t(size) : kOutOfRange;
-      const uint32_t alone = pair + 1 == a.n ? uint32_t(pair) * uint32_t(size) : kOutOfRange;
-      const bool any_alone = __builtin_amdgcn_ballot_w64(alone != kOutOfRange) != 0;
-      uint32_t cb[B];
+    constexpr int U = 4 / Q, kSteps = FM * (FO / B) * U;
+    const int half = lane >> 5;
+    const int size = a.out_type == I8CONV_FP32 ? 4 : 2;
+    uint32_t yp = uint32_t(a.ldy) * uint32_t(size), rp = uint32_t(a.ldr) * uint32_t(size);
+    asm volatile("" : "+s"(yp), "+s"(rp));  // (no products of them kept in registers across the sums)
+    struct Step {
+      int i, j, g0;  // first output block, row block, first quad
+    };
+    auto step_of = [&](int st) { return Step{st / U / FM * B, st / U % FM, st % U * Q}; };
+    // this lane's first channel in the tile; the step's first row in it
+    auto channel_of = [&](Step s) {
+      return wn * (32 * FO) + (kPair ? s.i * 32 + 2 * (lane & 31) : 32 * s.i + (lane & 31));
+    };
+    auto row0_of = [&](Step s) { return wm * TM + 32 * s.j + 8 * s.g0; };
+    // row of a lane's element e: its own part, and that of all lanes
+    auto row_of = [&](int e, uint32_t pitch) { return uint32_t(8 * (e / 4) + e % 4) * pitch; };
+    uint32_t own_y = uint32_t(4 * half) * yp, own_r = uint32_t(4 * half) * rp;
+    // (as values of their own: as part of a 64-bit multiply-add they tied the
+    // stores to the residual's registers, and so each to the stores before it)
+    asm volatile("" : "+v"(own_y), "+v"(own_r));
+    // A window over a step's rows, the first at 0: rows past the tile's last are
+    // out of its range, and so is the column of a channel past n.
+    auto window = [&](Step s, const void *base, int64_t ld, uint32_t pitch) {
+      const int w0 = row0_of(s), in = min(out_rows - w0, 8 * Q);
+      return make_rsrc(static_cast<const int8_t *>(base) + (out_row + w0) * ld * size,
+                       in > 0 && base ? uint32_t(in - 1) * pitch + uint32_t(a.n) * uint32_t(size) : 0u);
+    };
+    // 16-bit outputs leave two channels to a dword, at any alignment (buffer
+    // accesses need none).  Single blocks: of every two rows an even lane takes
+    // the first and its odd neighbour the second.  With n odd the last channel
+    // is alone.
+    const int odd = kPair ? 0 : lane & 1;
+    constexpr int W = kPair ? 4 * Q : 2 * Q;  // dwords
+    auto word_row = [&](int w, uint32_t pitch) { return row_of(kPair ? w : 2 * w, pitch); };
+    struct Columns {
+      uint32_t pair, alone, single[B];
+      bool any_alone;
+    };
+    auto columns_of = [&](Step s) {
+      const int ch = out_n + channel_of(s), pair = ch - odd;
+      Columns c;
+      c.pair = pair + 1 < a.n ? uint32_t(pair) * uint32_t(size) : kOutOfRange;
+      c.alone = pair + 1 == a.n ? uint32_t(pair) * uint32_t(size) : kOutOfRange;
+      c.any_alone = __builtin_amdgcn_ballot_w64(c.alone != kOutOfRange) != 0;
 #pragma unroll
-      for (int b = 0; b < B; ++b) cb[b] = ch + b < a.n ? uint32_t(ch + b) * uint32_t(size) : kOutOfRange;
-
-      // the residual, on its way while the sums are worked on
-      uint32_t res[B][4 * Q];
-      if (a.residual) {
-        if (size == 2) {
+      for (int b = 0; b < B; ++b)
+        c.single[b] = ch + b < a.n ? uint32_t(ch + b) * uint32_t(size) : kOutOfRange;
+      return c;
+    };
+    // the residual of a step, on its way while the sums are worked on
+    uint32_t res[B][4 * Q];
+    auto fetch = [&](Step s) {
+      const Columns c = columns_of(s);
+      const auto rr = window(s, a.residual, a.ldr, rp);
+      if (size == 2) {
+        const uint32_t at = own_r + uint32_t(odd) * rp;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          res[0][w] = __builtin_amdgcn_raw_buffer_load_b32(rr, c.pair + at + word_row(w, rp), 0, 0);
+        if (c.any_alone) {
 #pragma unroll
           for (int w = 0; w < W; ++w)
-            res[0][w] = __builtin_amdgcn_raw_buffer_load_b32(rr, cw + uint32_t(word_row(w)) * rp, 0, 0);
-          if (any_alone) {
-#pragma unroll
-            for (int w = 0; w < W; ++w)
-              res[0][w] |= __builtin_amdgcn_raw_buffer_load_b16(rr, alone + uint32_t(word_row(w)) * rp, 0, 0);
-          }
-        } else {
-#pragma unroll
-          for (int b = 0; b < B; ++b)
-#pragma unroll
-            for (int e = 0; e < 4 * Q; ++e)
-              res[b][e] = __builtin_amdgcn_raw_buffer_load_b32(rr, cb[b] + uint32_t(row_of(e)) * rp, 0, 0);
+            res[0][w] |= __builtin_amdgcn_raw_buffer_load_b16(rr, c.alone + at + word_row(w, rp), 0, 0);
         }
+      } else {
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+          for (int e = 0; e < 4 * Q; ++e)
+            res[b][e] = __builtin_amdgcn_raw_buffer_load_b32(rr, c.single[b] + own_r + row_of(e, rp), 0, 0);
       }
-
+    };
+    // a step's row and weight scales and biases
+    struct Scales {
+      v4f xs[Q];
+      float ws[B], bias[B], ws2[B], bias2[B];
+    };
+    auto scales_of = [&](Step s) {
+      const int ct = channel_of(s);
+      const float *const xs = pr + 2 * BN + row0_of(s) + 4 * half;
+      Scales f;
+#pragma unroll
+      for (int q = 0; q < Q; ++q) f.xs[q] = *reinterpret_cast<const v4f *>(xs + 8 * q);
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        f.ws[b] = pr[ct + b], f.bias[b] = pr[BN + ct + b];
+        if constexpr (kGated) f.ws2[b] = pr[BO + ct + b], f.bias2[b] = pr[BN + BO + ct + b];
+      }
+      return f;
+    };
+    // step s with its sums sg (and su, the other halves')
+    auto finish = [&](Step s, const v4i (&sg)[B][Q], const v4i (&su)[B][Q]) {
+      const Scales f = scales_of(s);
+      if (a.residual) fetch(s);
+      const Columns c = columns_of(s);
+      const auto yr = window(s, a.y, a.ldy, yp);
       float v[B][4 * Q];
 #pragma unroll
       for (int b = 0; b < B; ++b) {
-        const float ws = pr[ct + b], bias = pr[BN + ct + b];
         float u[4 * Q];
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          const v4f xs = *reinterpret_cast<const v4f *>(pr + 2 * BN + r0 + 8 * q);
+        for (int q = 0; q < Q; ++q)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[b][4 * q + e] = fmaf(float(sg[b][q][e]) * xs[e], ws, bias);
-          if constexpr (kGated) {
-            const float ws2 = pr[BO + ct + b], bias2 = pr[BN + BO + ct + b];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              u[4 * q + e] = fmaf(float(su[b][q][e]) * xs[e], ws2, bias2);
+          for (int e = 0; e < 4; ++e) {
+            v[b][4 * q + e] = fmaf(float(sg[b][q][e]) * f.xs[q][e], f.ws[b], f.bias[b]);
+            if constexpr (kGated)
+              u[4 * q + e] = fmaf(float(su[b][q][e]) * f.xs[q][e], f.ws2[b], f.bias2[b]);
           }
-        }
         activate(v[b], a.activation);
         if constexpr (kGated) {
 #pragma unroll
@@ -419,42 +462,58 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
         }
       }
       if (size == 4) {
+        if (a.residual) {
+#pragma unroll
+          for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int e = 0; e < 4 * Q; ++e) v[b][e] += bits_f32(res[b][e]);
+        }
 #pragma unroll
         for (int e = 0; e < 4 * Q; ++e) {
-          if (a.residual) {
+          const uint32_t row = own_y + row_of(e, yp);
+          if constexpr (kPair)
+            __builtin_amdgcn_raw_buffer_store_b64(v2u{f32_bits(v[0][e]), f32_bits(v[1][e])}, yr, c.pair + row, 0, 0);
+          else
+            __builtin_amdgcn_raw_buffer_store_b32(f32_bits(v[0][e]), yr, c.single[0] + row, 0, 0);
+        }
+        if (kPair && c.any_alone) {
 #pragma unroll
-            for (int b = 0; b < B; ++b) v[b][e] += bits_f32(res[b][e]);
-          }
-          const uint32_t row = uint32_t(row_of(e)) * yp;
-          if constexpr (kPair) {
-            __builtin_amdgcn_raw_buffer_store_b64(v2u{f32_bits(v[0][e]), f32_bits(v[1][e])}, yr, cw + row, 0, 0);
-            if (any_alone)
-              __builtin_amdgcn_raw_buffer_store_b32(f32_bits(v[0][e]), yr, alone + row, 0, 0);
-          } else {
-            __builtin_amdgcn_raw_buffer_store_b32(f32_bits(v[0][e]), yr, cb[0] + row, 0, 0);
-          }
+          for (int e = 0; e < 4 * Q; ++e)
+            __builtin_amdgcn_raw_buffer_store_b32(f32_bits(v[0][e]), yr, c.alone + own_y + row_of(e, yp), 0, 0);
         }
         return;
       }
+      float lo[W], hi[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if constexpr (kPair) {
+          lo[w] = v[0][w], hi[w] = v[B - 1][w];
+        } else {
+          const float got = neighbour(odd ? v[0][2 * w] : v[0][2 * w + 1]);
+          lo[w] = odd ? got : v[0][2 * w];
+          hi[w] = odd ? v[0][2 * w + 1] : got;
+        }
+      }
       auto store16 = [&](auto kind) {  // (the type once for all, not per value)
         constexpr int T = decltype(kind)::value;
+        if (a.residual) {
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            lo[w] += from_half(res[0][w] & 0xffffu, T);
+            hi[w] += from_half(res[0][w] >> 16, T);
+          }
+        }
+        const uint32_t at = own_y + uint32_t(odd) * yp;
+        uint32_t word[W];
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          float lo, hi;
-          if constexpr (kPair) {
-            lo = v[0][w], hi = v[B - 1][w];
-          } else {
-            const float got = neighbour(odd ? v[0][2 * w] : v[0][2 * w + 1]);
-            lo = odd ? got : v[0][2 * w];
-            hi = odd ? v[0][2 * w + 1] : got;
-          }
-          if (a.residual) {
-            lo += from_half(res[0][w] & 0xffffu, T);
-            hi += from_half(res[0][w] >> 16, T);
-          }
-          const uint32_t word = to_halves(lo, hi, T), row = uint32_t(word_row(w)) * yp;
-          __builtin_amdgcn_raw_buffer_store_b32(word, yr, cw + row, 0, 0);
-          if (any_alone) __builtin_amdgcn_raw_buffer_store_b16(uint16_t(word), yr, alone + row, 0, 0);
+          word[w] = to_halves(lo[w], hi[w], T);
+          __builtin_amdgcn_raw_buffer_store_b32(word[w], yr, c.pair + at + word_row(w, yp), 0, 0);
+        }
+        if (c.any_alone) {
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            __builtin_amdgcn_raw_buffer_store_b16(uint16_t(word[w]), yr, c.alone + at + word_row(w, yp), 0, 0);
         }
       };
       if (a.out_type == I8CONV_BF16)
@@ -462,36 +521,119 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
       else
         store16(Set<I8CONV_FP16>{});
     };
+    // All steps without a loop: 16-bit outputs whose channels all have a partner,
+    // under an activation of few instructions.  A wave starts an instruction in
+    // eight cycles whatever it is, so the epilogue takes as long as it has
+    // instructions: without the loop's moves and branches 8192 x 1024 -> 4096 took
+    // 42.5 us for 49.4, gated with silu 83.7 for 94.8, 32768 rows of 64 experts
+    // 1024 -> 2048 120 for 139.  (fp32 outputs in the same code: 27.4 us for 28.8 of
+    // 2048 x 1024 -> 8192, but 127 for 120 of the experts' bf16, by spills.)
+    auto finish_pairs = [&](auto pairs) {
+#pragma unroll
+      for (int i = 0; i < decltype(pairs)::value; ++i) {
+        const int ct = wn * (32 * FO) + 64 * i + 2 * (lane & 31);
+        const uint32_t col = out_n + ct < a.n ? uint32_t(out_n + ct) * 2u : kOutOfRange;
+        float ws[2], bias[2], ws2[2], bias2[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          ws[b] = pr[ct + b], bias[b] = pr[BN + ct + b];
+          if constexpr (kGated) ws2[b] = pr[BO + ct + b], bias2[b] = pr[BN + BO + ct + b];
+        }
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            __builtin_amdgcn_sched_barrier(0);
+            // rows w0 .. w0 + 15 of the tile
+            const int w0 = wm * TM + 32 * j + 16 * g, in = min(out_rows - w0, 16);
+            auto rows_of = [&](const void *base, int64_t ld, uint32_t pitch) {
+              return make_rsrc(static_cast<const int8_t *>(base) + (out_row + w0) * ld * 2,
+                               in > 0 ? uint32_t(in - 1) * pitch + uint32_t(a.n) * 2u : 0u);
+            };
+            uint32_t rs[8];
+            if (a.residual) {
+              const auto rr = rows_of(a.residual, a.ldr, rp);
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                rs[e] = __builtin_amdgcn_raw_buffer_load_b32(rr, col + own_r + row_of(e, rp), 0, 0);
+            }
+            v4f xs[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              xs[q] = *reinterpret_cast<const v4f *>(pr + 2 * BN + w0 + 8 * q + 4 * half);
+            float v[16];  // even channel, odd channel of each row
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+              for (int b = 0; b < 2; ++b)
+                v[2 * e + b] = fmaf(float(acc[2 * i + b][j][8 * g + e]) * xs[e / 4][e % 4], ws[b], bias[b]);
+            activate<16, false>(v, a.activation);
+            if constexpr (kGated) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                  v[2 * e + b] *= fmaf(float(acc[FO + 2 * i + b][j][8 * g + e]) * xs[e / 4][e % 4], ws2[b],
+                                       bias2[b]);
+            }
+            const auto yr = rows_of(a.y, a.ldy, yp);
+            auto store = [&](auto kind) {
+              constexpr int T = decltype(kind)::value;
+              if (a.residual) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  v[2 * e] += from_half(rs[e] & 0xffffu, T);
+                  v[2 * e + 1] += from_half(rs[e] >> 16, T);
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                __builtin_amdgcn_raw_buffer_store_b32(to_halves(v[2 * e], v[2 * e + 1], T), yr,
+                                                      col + own_y + row_of(e, yp), 0, 0);
+            };
+            if (a.out_type == I8CONV_BF16)
+              store(Set<I8CONV_BF16>{});
+            else
+              store(Set<I8CONV_FP16>{});
+          }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
     if constexpr (KG == 1) {
       // the next tile's copies go out before this tile's stores
       if (again) {
         setup(t);
         prologue(slot ^ 1);
       }
-      // One copy of the code for all blocks: a step's sums are moved into
-      // registers of their own first.  (Unrolled over the blocks it took 112 KB
-      // and spilled 104 registers: 1024 rows of 8 tiles each, 16384 x 2048 ->
-      // 8192, 434 us; 270 with one output type's code only.)
-      constexpr int U = 4 / Q, kSteps = FM * (FO / B) * U;
+      bool loop = !idle;
+      if constexpr (kPair) {
+        if (loop && size == 2 && a.activation != I8CONV_ACT_GELU && (out_n + BO <= a.n || a.n % 2 == 0)) {
+          loop = false;
+          finish_pairs(Set<FO / 2>{});
+        }
+      }
+      // The rest in one copy of the code for all blocks: a step's sums are moved
+      // into registers of their own first.
 #pragma unroll 1
-      for (int st = idle ? kSteps : 0; st < kSteps; ++st) {
+      for (int st = loop ? 0 : kSteps; st < kSteps; ++st) {
+        const Step now = step_of(st);
         v4i sg[B][Q], su[B][Q];
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
           if (st != c) continue;
           asm volatile("" ::: "memory");  // a branch: selects would run through every block's registers
-          const int j = c / U % FM, i = c / U / FM * B, g0 = c % U * Q;
+          const Step k = step_of(c);
 #pragma unroll
           for (int b = 0; b < B; ++b)
 #pragma unroll
             for (int q = 0; q < Q; ++q)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                sg[b][q][e] = acc[i + b][j][4 * (g0 + q) + e];
-                if constexpr (kGated) su[b][q][e] = acc[FO + i + b][j][4 * (g0 + q) + e];
+                sg[b][q][e] = acc[k.i + b][k.j][4 * (k.g0 + q) + e];
+                if constexpr (kGated) su[b][q][e] = acc[FO + k.i + b][k.j][4 * (k.g0 + q) + e];
               }
         }
-        finish(st / U / FM * B, st / U % FM, st % U * Q, sg, su);
+        finish(now, sg, su);
       }
     } else {
       // each wave's sums go to the first stage buffers (every wave has read
@@ -519,19 +661,18 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
         for (int g = 1; g < KG; ++g) sum += *reinterpret_cast<const v4u *>(part_of(g, b, q));
         return __builtin_bit_cast(v4i, sum);
       };
-      constexpr int U = 4 / Q, kSteps = FM * (FO / B) * U;
 #pragma unroll 1
       for (int st = group; st < kSteps; st += KG) {
-        const int j = st / U % FM, i = st / U / FM * B, g0 = st % U * Q;
+        const Step now = step_of(st);
         v4i sg[B][Q], su[B][Q];
 #pragma unroll
         for (int b = 0; b < B; ++b)
 #pragma unroll
           for (int q = 0; q < Q; ++q) {
-            sg[b][q] = total(i + b, j, g0 + q);
-            if constexpr (kGated) su[b][q] = total(FO + i + b, j, g0 + q);
+            sg[b][q] = total(now.i + b, now.j, now.g0 + q);
+            if constexpr (kGated) su[b][q] = total(FO + now.i + b, now.j, now.g0 + q);
           }
-        finish(i, j, g0, sg, su);
+        finish(now, sg, su);
       }
       if (again) {
         barrier_lds();

@@ -106,17 +106,18 @@ __device__ __forceinline__ void store_values4(void *p, int64_t i, int type, v4f 
   *reinterpret_cast<v2u *>(static_cast<uint16_t *>(p) + i) = h;
 }
 
-// The activation of N values, of a wave-uniform kind.  relu keeps NaN.
+// The activation of N values, of a wave-uniform kind (without kErf not
+// I8CONV_ACT_GELU).  relu keeps NaN.
 // gelu_tanh and silu are both v times the logistic function of a polynomial:
 // 0.5 (1 + tanh(z / 2)) = 1 / (1 + 2^(-z log2 e)); their exponentials overflow
 // to infinity for large negative values and the product is then -0, the limit.
-template <int N>
+template <int N, bool kErf = true>
 __device__ __forceinline__ void activate(float (&v)[N], int kind) {
   if (kind == I8CONV_ACT_NONE) return;
   if (kind == I8CONV_ACT_RELU) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
-  } else if (kind == I8CONV_ACT_GELU) {
+  } else if (kErf && kind == I8CONV_ACT_GELU) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678f));
   } else {

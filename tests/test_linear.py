@@ -522,6 +522,25 @@ def test_linear_last_channel_alone(odd, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("n", [514, 515, 1024])
+@pytest.mark.parametrize("rows", [700, 2500, 9000])
+def test_linear_both_epilogues(rows, n, act):
+    # whole and partial column tiles, with and without a last channel alone,
+    # several tiles in turn to a workgroup
+    run_linear(rows, 144, n, y="fp16", act=act, bias=True, residual=True, strides=(0, n + 6, n + 2))
+    run_linear(rows, 144, n, act=act, gated=True, residual=n % 2 == 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [130, 131, 768])
+def test_experts_both_epilogues(n):
+    counts = [300, 0, 5, 257, 1, 600, 256, 90]
+    run_experts(counts, 144, n, tokens=400, act="silu", gated=True)
+    run_experts(counts, 144, n, tokens=400, bias=True, y="fp16")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("experts,choices", [(0, 0), (8, 2)])
 @pytest.mark.parametrize("tokens", [1, 37])
 def test_feed_forward_example(experts, choices, tokens, capsys):
