@@ -295,9 +295,10 @@ int done(const char *what) {
 
 }  // namespace
 
-// Lists from this many ids on take the two launches: 131072 ids of 128 experts
-// 64 us with a workgroup per expert, which reads all of them twice.
-constexpr int kRouteLong = 8192;
+// Lists from this many ids on take the two launches.  128 experts, us in one
+// launch, where a workgroup per expert reads all ids twice, and in two: 8192 ids
+// 6.9 and 8.3, 16384 10.0 and 8.8, 131072 56.2 and 9.7.
+constexpr int kRouteLong = 16384;
 bool route_long(int64_t ids, int experts) { return ids >= kRouteLong && experts <= kRouteThreads; }
 
 size_t route_workspace(int64_t ids, int experts) {

@@ -15,6 +15,10 @@
 //
 // By expert: a workgroup row (blockIdx.y) takes the y-th of the experts that
 // have rows.
+//
+// One row 4096 -> 4096 8.2 us (2.0 TB/s: a launch, the memory's latency and the
+// sums take most of it), 16 rows 4096 -> 12288 gated 27.0 us (3.7 TB/s), 148 rows
+// of 60 experts 1040 -> 720 gated 14.7 us (6.1 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

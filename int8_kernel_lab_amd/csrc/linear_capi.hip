@@ -146,8 +146,7 @@ int run(const i8conv_linear_shape &s, const void *input, const float *input_scal
   a.experts = s.experts;
   a.activation = s.activation;
   a.out_type = s.output_type;
-  a.vec4 = linear_vec_ok(output, a.ldy, a.n, size, 4) &&
-           (!residual || linear_vec_ok(residual, a.ldr, a.n, size, 4));
+  a.vec4 = linear_vec_ok(output, a.ldy, a.n, size, 4);
   const RowsPlan plan = plan_rows(s, input);
   a.x_type = s.input_type;
   if (plan.fused || s.input_type == I8CONV_INT8) {

@@ -429,6 +429,14 @@ def test_route(tokens, choices, experts, dropped):
     assert places.reshape(-1).tolist() == want[2]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,choices,experts,dropped", [
+    (16383, 1, 1024, 0.05), (16384, 1, 1024, 0), (16385, 1, 257, 0.4), (4097, 4, 2, 0), (5000, 7, 1000, 1.0),
+    (4100, 4, 1025, 0.1)])
+def test_route_around_two_launches(tokens, choices, experts, dropped):
+    test_route(tokens, choices, experts, dropped)
+
+
 def run_experts(counts, k, n, x="bf16", y="bf16", act="none", gated=False, bias=False, tokens=None,
                 spare=0, seed=9, strides=(0, 0), offset=0):
     """Rows of `counts` per expert; gathered from `tokens` rows, or in place."""
