@@ -68,20 +68,20 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(const int32_t *ids
     for (int i = total + int(threadIdx.x); i < count; i += kRouteThreads) sources[i] = -1;
 }
 
-// Long lists, two launches over parts of kPartIds ids.  First the experts'
+// Long lists, two launches over parts of U ids per thread.  First the experts'
 // counts of each part.  Then a workgroup per part has the part's first row of
 // every expert from the counts of the parts before, and the rows of its waves'
 // segments from counts of its own; a wave ranks 64 ids at a time by the lanes
 // with the same id, one ballot per bit of an id.
-constexpr int kPartIds = 4096, kWaveIds = kPartIds / kRouteWaves;
+template <int U>
 __global__ __launch_bounds__(kRouteThreads) void route_count_kernel(const int32_t *ids, int count,
                                                                    int experts, int32_t *counts) {
   extern __shared__ int sum[];
   for (int e = threadIdx.x; e < experts; e += kRouteThreads) sum[e] = 0;
   __syncthreads();
-  const int begin = int(blockIdx.x) * kPartIds;
+  const int begin = int(blockIdx.x) * U * kRouteThreads;
 #pragma unroll
-  for (int u = 0; u < kPartIds / kRouteThreads; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int i = begin + u * kRouteThreads + int(threadIdx.x);
     const int id = i < count ? ids[i] : -1;
     if (id >= 0 && id < experts) atomicAdd(&sum[id], 1);
@@ -91,38 +91,49 @@ __global__ __launch_bounds__(kRouteThreads) void route_count_kernel(const int32_
     counts[int64_t(blockIdx.x) * experts + e] = sum[e];
 }
 
+template <int U>
 __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(
     const int32_t *ids, int count, int choices, int experts, int id_bits, const int32_t *counts,
     int32_t *offsets, int32_t *sources, int32_t *places) {
-  extern __shared__ int next[];  // [waves][experts], then the waves' totals
-  int *const totals = next + kRouteWaves * experts;
+  // [waves][experts], each expert's rows before this part and in all, the waves' totals
+  extern __shared__ int next[];
+  int *const before_of = next + kRouteWaves * experts, *const all_of = before_of + experts;
+  int *const totals = all_of + experts;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int part = blockIdx.x, parts = gridDim.x;
-  const int begin = part * kPartIds + wave * kWaveIds;
-  int id[kWaveIds / 64];
+  const int begin = part * U * kRouteThreads + wave * U * 64;
+  int id[U];
 #pragma unroll
-  for (int u = 0; u < kWaveIds / 64; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int i = begin + u * 64 + lane;
     id[u] = i < count ? ids[i] : -1;
     if (id[u] >= experts) id[u] = -1;
   }
-  for (int e = threadIdx.x; e < kRouteWaves * experts; e += kRouteThreads) next[e] = 0;
-  __syncthreads();
-  // (whole numbers: the order of the additions does not show)
-#pragma unroll
-  for (int u = 0; u < kWaveIds / 64; ++u)
-    if (id[u] >= 0) atomicAdd(&next[wave * experts + id[u]], 1);
-  // expert threadIdx.x (experts <= kRouteThreads): its rows before this part and in all
-  const int e = threadIdx.x;
+  // expert threadIdx.x % experts (experts <= kRouteThreads), of every groups-th part
+  const int groups = kRouteThreads / experts, mine = int(threadIdx.x) % experts;
   int before = 0, all = 0;
-  if (e < experts) {
-#pragma unroll 8
-    for (int p = 0; p < parts; ++p) {
-      const int c = counts[int64_t(p) * experts + e];
+  if (int(threadIdx.x) < groups * experts) {
+#pragma unroll 4
+    for (int p = int(threadIdx.x) / experts; p < parts; p += groups) {
+      const int c = counts[int64_t(p) * experts + mine];
       before += p < part ? c : 0;
       all += c;
     }
   }
+  for (int i = threadIdx.x; i < (kRouteWaves + 2) * experts; i += kRouteThreads) next[i] = 0;
+  __syncthreads();
+  // (whole numbers: the order of the additions does not show)
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (id[u] >= 0) atomicAdd(&next[wave * experts + id[u]], 1);
+  if (all > 0) {
+    atomicAdd(&before_of[mine], before);
+    atomicAdd(&all_of[mine], all);
+  }
+  __syncthreads();
+  const int e = threadIdx.x;
+  before = e < experts ? before_of[e] : 0;
+  all = e < experts ? all_of[e] : 0;
   int sum = all;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -148,7 +159,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_place_kernel(
   if (part == 0 && e == 0) offsets[experts] = total;
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < kWaveIds / 64; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int i = begin + u * 64 + lane;
     const bool live = id[u] >= 0;
     uint64_t same = __ballot(live);
@@ -296,14 +307,41 @@ int done(const char *what) {
 }  // namespace
 
 // Lists from this many ids on take the two launches.  128 experts, us in one
-// launch, where a workgroup per expert reads all ids twice, and in two: 8192 ids
-// 6.9 and 8.3, 16384 10.0 and 8.8, 131072 56.2 and 9.7.
+// launch, where a workgroup per expert reads all ids twice, and in two: 16384 ids
+// 10.0 and 7.4, 131072 56.2 and 8.3; 8192 6.9 in one, less than two launches take.
 constexpr int kRouteLong = 16384;
 bool route_long(int64_t ids, int experts) { return ids >= kRouteLong && experts <= kRouteThreads; }
 
-size_t route_workspace(int64_t ids, int experts) {
-  return route_long(ids, experts) ? size_t((ids + kPartIds - 1) / kPartIds) * size_t(experts) * 4 : 0;
+// Ids per thread: every part reads the counts of all parts, so that longer lists
+// take larger ones (us with 2 and with 8: 16384 ids of 128 experts 7.4 and 12.2,
+// 131072 8.3 and 13.3, 524288 12.3 and 14.2, 1048576 21.1 and 16.0).
+int route_ids_per_thread(int64_t ids) { return ids <= 1 << 19 ? 2 : 8; }
+int route_parts(int64_t ids) {
+  const int64_t per = int64_t(route_ids_per_thread(ids)) * kRouteThreads;
+  return int((ids + per - 1) / per);
 }
+
+size_t route_workspace(int64_t ids, int experts) {
+  return route_long(ids, experts) ? size_t(route_parts(ids)) * size_t(experts) * 4 : 0;
+}
+
+namespace {
+template <int U>
+int launch_route_long(const int32_t *ids, int count, int choices, int experts, int32_t *offsets,
+                      int32_t *sources, int32_t *places, int32_t *counts, hipStream_t s) {
+  const dim3 parts(unsigned(route_parts(count)));
+  int id_bits = 0;
+  while ((1 << id_bits) < experts) ++id_bits;
+  I8_LAUNCH(route_count_kernel<U>, parts, dim3(kRouteThreads), size_t(experts) * 4, s, ids, count,
+            experts, counts);
+  const size_t lds = size_t(kRouteWaves + 2) * experts * 4 + kRouteWaves * 4;
+  static LdsLimit limit;
+  if (const int rc = limit.raise(route_place_kernel<U>, lds); rc != I8CONV_OK) return rc;
+  I8_LAUNCH(route_place_kernel<U>, parts, dim3(kRouteThreads), lds, s, ids, count, choices, experts,
+            id_bits, counts, offsets, sources, places);
+  return done("route launch");
+}
+}  // namespace
 
 int launch_route(const int32_t *ids, int tokens, int choices, int experts, int32_t *offsets,
                  int32_t *sources, int32_t *places, void *workspace, void *stream) {
@@ -315,17 +353,9 @@ int launch_route(const int32_t *ids, int tokens, int choices, int experts, int32
     return done("route launch");
   }
   int32_t *const counts = static_cast<int32_t *>(workspace);
-  const unsigned parts = unsigned((int64_t(count) + kPartIds - 1) / kPartIds);
-  int id_bits = 0;
-  while ((1 << id_bits) < experts) ++id_bits;
-  I8_LAUNCH(route_count_kernel, dim3(parts), dim3(kRouteThreads), size_t(experts) * 4, s, ids, count,
-            experts, counts);
-  const size_t lds = size_t(kRouteWaves) * experts * 4 + kRouteWaves * 4;
-  static LdsLimit limit;
-  if (const int rc = limit.raise(route_place_kernel, lds); rc != I8CONV_OK) return rc;
-  I8_LAUNCH(route_place_kernel, dim3(parts), dim3(kRouteThreads), lds, s, ids, count, choices, experts,
-            id_bits, counts, offsets, sources, places);
-  return done("route launch");
+  return route_ids_per_thread(count) == 2
+             ? launch_route_long<2>(ids, count, choices, experts, offsets, sources, places, counts, s)
+             : launch_route_long<8>(ids, count, choices, experts, offsets, sources, places, counts, s);
 }
 
 int launch_combine(const void *x, int in_type, const int32_t *places, const float *weights,

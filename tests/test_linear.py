@@ -432,7 +432,7 @@ def test_route(tokens, choices, experts, dropped):
 @pytest.mark.gpu
 @pytest.mark.parametrize("tokens,choices,experts,dropped", [
     (16383, 1, 1024, 0.05), (16384, 1, 1024, 0), (16385, 1, 257, 0.4), (4097, 4, 2, 0), (5000, 7, 1000, 1.0),
-    (4100, 4, 1025, 0.1)])
+    (4100, 4, 1025, 0.1), (300000, 2, 37, 0.02)])
 def test_route_around_two_launches(tokens, choices, experts, dropped):
     test_route(tokens, choices, experts, dropped)
 
