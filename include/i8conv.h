@@ -262,9 +262,10 @@ typedef enum i8conv_activation {
   I8CONV_ACT_SILU = 4       /* v / (1 + exp(-v)) */
 } i8conv_activation;
 
-/* A linear layer.  `rows` may be 0 (nothing is launched) and is below 2^29;
- * inputs % 16 == 0 and < 2^17; the weights of one matrix (outputs, or 2 * outputs where gated,
- * times inputs) below 2^31 bytes, outputs below 2^24.  Strides are elements
+/* A linear layer.  `rows` may be 0 (nothing is launched) and is below 2^29, as
+ * is `routed`; inputs % 16 == 0 and < 2^17; the weights of one matrix (outputs,
+ * or 2 * outputs where gated, times inputs) are below 2^31 bytes, outputs below
+ * 2^24, rows of the output times outputs below 2^39.  Strides are elements
  * between rows, 0 for packed rows; that of an int8 input is a multiple of 16
  * below 2^23, those of output and residual are below 2^24. */
 typedef struct i8conv_linear_shape {

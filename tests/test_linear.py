@@ -530,6 +530,61 @@ def test_linear_last_channel_alone(odd, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,choices", [(1, 4), (3, 2), (90, 4), (5000, 4)])
+def test_layer_of_experts_replays_from_a_graph(tokens, choices):
+    # the chain captured once, replayed on other tokens and choices with eager
+    # passes between: the same bytes as eager each time
+    say(f"[gpu] graph of a layer of experts, {tokens} tokens of {choices}")
+    k, n, experts, rows = 144, 80, 16, tokens * choices
+    g = _gen(12)
+    w1, w2 = _codes(g, experts, 2 * n, k), _codes(g, experts, k, n)
+    s1 = torch.full((experts, 2 * n), 2e-3, device="cuda")
+    s2 = torch.full((experts, k), 2e-3, device="cuda")
+    x = torch.zeros(tokens, k, device="cuda", dtype=torch.bfloat16)
+    ids = torch.zeros(tokens, choices, device="cuda", dtype=torch.int32)
+    weights = torch.zeros(tokens, choices, device="cuda")
+    up = lab.LinearShape(tokens, k, n, "bf16", "bf16", gated=True, activation="silu", experts=experts, routed=rows)
+    down = lab.LinearShape(rows, n, k, "bf16", "bf16", experts=experts, routed=rows)
+    route, combine = lab.RouteShape(tokens, choices, experts), lab.CombineShape(tokens, choices, k)
+    need = max(lab.linear_workspace_bytes(up), lab.linear_workspace_bytes(down),
+               lab.route_workspace_bytes(route))
+
+    def buffers():
+        return dict(o=torch.zeros(experts + 1, device="cuda", dtype=torch.int32),
+                    s=torch.zeros(rows, device="cuda", dtype=torch.int32),
+                    p=torch.zeros(rows, device="cuda", dtype=torch.int32),
+                    h=torch.zeros(rows, n, device="cuda", dtype=torch.bfloat16),
+                    z=torch.zeros(rows, k, device="cuda", dtype=torch.bfloat16),
+                    y=torch.zeros(tokens, k, device="cuda", dtype=torch.bfloat16), w=_ws(max(need, 1)))
+
+    def run(b):
+        st = _stream()
+        lab.launch_route(route, _p(ids), _p(b["o"]), _p(b["s"]), _p(b["p"]), _p(b["w"]), need, st)
+        lab.launch_expert_linear(up, _p(x), None, _p(w1), _p(s1), None, _p(b["o"]), _p(b["s"]), _p(b["h"]),
+                                 _p(b["w"]), need, st)
+        lab.launch_expert_linear(down, _p(b["h"]), None, _p(w2), _p(s2), None, _p(b["o"]), None, _p(b["z"]),
+                                 _p(b["w"]), need, st)
+        lab.launch_combine(combine, _p(b["z"]), _p(b["p"]), _p(weights), _p(x), _p(b["y"]), st)
+
+    eager, captured = buffers(), buffers()
+    run(captured)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(captured)
+    for turn in range(4):
+        x.copy_(_normal(g, tokens, k))
+        ids.copy_(torch.randint(-1, experts, (tokens, choices), generator=g, device="cuda"))
+        weights.copy_(_normal(g, tokens, choices))
+        graph.replay()
+        torch.cuda.synchronize()
+        run(eager)
+        torch.cuda.synchronize()
+        assert torch.equal(eager["y"], captured["y"]), turn
+        assert eager["y"].float().isfinite().all() and not torch.equal(eager["y"], x)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
 @pytest.mark.parametrize("n", [514, 515, 1024])
 @pytest.mark.parametrize("rows", [700, 2500, 9000])
