@@ -604,6 +604,30 @@ def test_experts_both_epilogues(n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("last", [3, 50, 300])
+def test_experts_weights_past_32_bits(last):
+    # 36 matrices of 2^27 bytes: the last begin past 2^32, in each kernel
+    run_experts([2] + [0] * 34 + [last], 8192, 16384, tokens=20)
+
+
+@pytest.mark.gpu
+def test_combine_rows_past_32_bits():
+    tokens, choices, n = 40000, 8, 8192  # 2.6e9 values
+    say("[gpu] combine of 2.6e9 values")
+    g = _gen(13)
+    rows = tokens * choices
+    v = torch.empty((rows, n), device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    places = torch.randperm(rows, generator=g, device="cuda").to(torch.int32).view(tokens, choices)
+    weights = torch.rand((tokens, choices), generator=g, device="cuda")
+    out = torch.empty((tokens, n), device="cuda", dtype=torch.bfloat16)
+    lab.launch_combine(lab.CombineShape(tokens, choices, n), _p(v), _p(places), _p(weights), None,
+                       _p(out), _stream())
+    for part in (slice(0, 50), slice(tokens - 50, tokens)):
+        terms = v[places[part].long()].double() * weights[part][..., None].double()
+        assert_close(out[part], terms.sum(1), terms.abs().sum(1), "bf16")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("experts,choices", [(0, 0), (8, 2)])
 @pytest.mark.parametrize("tokens", [1, 37])
 def test_feed_forward_example(experts, choices, tokens, capsys):
