@@ -30,10 +30,9 @@ const TileCost kTiles[] = {
     {kTile128x64Pair, 128, 64, 1, 2, 3, false, true, 0.60, 0.76, 3.0},
 };
 
-// Whole tiles and parts of one (which take about kPart of one's time) as rounds
-// of the chip, the last of them as full as it is.
-constexpr double kPart = 0.8;
-
+// Row tiles as rounds of the chip, the last of them as full as it is.  (A part of
+// a tile counts as a whole one: at 0.8 of it the choice for 300 drawn layers by
+// expert lay 3.7 % from the best tile in the mean, so 1.6 %.)
 double cost(const TileCost &t, double row_tiles, int64_t wide, int64_t k) {
   const double tiles = row_tiles * double((wide + t.bn - 1) / t.bn);
   const double slots = 256.0 * t.per_unit, rounds = std::floor(tiles / slots);
@@ -73,7 +72,7 @@ int plan_linear_tile(int64_t rows, int64_t experts, int64_t n, int64_t k, bool g
     if (experts) {
       // each group ends in a part of a tile, in the mean half of one
       const double groups = double(std::min(experts, rows));
-      row_tiles = std::max(0.0, double(rows) / t.bm - groups / 2) + kPart * groups;
+      row_tiles = std::max(0.0, double(rows) / t.bm - groups / 2) + groups;
     }
     const double us = cost(t, row_tiles, gated ? 2 * n : n, k);
     if (us < least) least = us, best = t.tile;
