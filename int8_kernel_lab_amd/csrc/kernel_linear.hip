@@ -534,17 +534,17 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
     // under an activation of few instructions.  A wave starts an instruction in
     // eight cycles whatever it is, so the epilogue takes as long as it has
     // instructions: without the loop's moves and branches 8192 x 1024 -> 4096 took
-    // 42.5 us for 49.4, gated with silu 83.7 for 94.8, 32768 rows of 64 experts
-    // 1024 -> 2048 120 for 139.  (fp32 outputs in the same code: 27.4 us for 28.8 of
-    // 2048 x 1024 -> 8192, but 127 for 120 of the experts' bf16, by spills.)
-    auto finish_pairs = [&](auto pairs) {
+    // 42.5 us for 49.4, gated with silu 83.7 for 94.8 (256 rows), 1000 x 1024 -> 4096
+    // 14.4 for 16.3 (128), 32768 rows of 64 experts 1024 -> 2048 120 for 139.
+    auto finish_straight = [&](auto residual) {
 #pragma unroll
-      for (int i = 0; i < decltype(pairs)::value; ++i) {
-        const int ct = wn * (32 * FO) + 64 * i + 2 * (lane & 31);
-        const uint32_t col = out_n + ct < a.n ? uint32_t(out_n + ct) * 2u : kOutOfRange;
-        float ws[2], bias[2], ws2[2], bias2[2];
+      for (int i = 0; i < FO / B; ++i) {
+        const int ct = wn * (32 * FO) + 32 * B * i + B * (lane & 31), pair = out_n + ct - odd;
+        const uint32_t col = pair < a.n ? uint32_t(pair) * 2u : kOutOfRange;
+        const uint32_t at_y = col + own_y + uint32_t(odd) * yp, at_r = col + own_r + uint32_t(odd) * rp;
+        float ws[B], bias[B], ws2[B], bias2[B];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < B; ++b) {
           ws[b] = pr[ct + b], bias[b] = pr[BN + ct + b];
           if constexpr (kGated) ws2[b] = pr[BO + ct + b], bias2[b] = pr[BN + BO + ct + b];
         }
@@ -559,46 +559,54 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
               return make_rsrc(static_cast<const int8_t *>(base) + (out_row + w0) * ld * 2,
                                in > 0 ? uint32_t(in - 1) * pitch + uint32_t(a.n) * 2u : 0u);
             };
-            uint32_t rs[8];
-            if (a.residual) {
+            uint32_t rs[4 * B];
+            if constexpr (residual.value) {
               const auto rr = rows_of(a.residual, a.ldr, rp);
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                rs[e] = __builtin_amdgcn_raw_buffer_load_b32(rr, col + own_r + row_of(e, rp), 0, 0);
+              for (int w = 0; w < 4 * B; ++w)
+                rs[w] = __builtin_amdgcn_raw_buffer_load_b32(rr, at_r + word_row(w, rp), 0, 0);
             }
             v4f xs[2];
 #pragma unroll
             for (int q = 0; q < 2; ++q)
               xs[q] = *reinterpret_cast<const v4f *>(pr + 2 * BN + w0 + 8 * q + 4 * half);
-            float v[16];  // even channel, odd channel of each row
+            float v[8 * B];  // of each row
 #pragma unroll
             for (int e = 0; e < 8; ++e)
 #pragma unroll
-              for (int b = 0; b < 2; ++b)
-                v[2 * e + b] = fmaf(float(acc[2 * i + b][j][8 * g + e]) * xs[e / 4][e % 4], ws[b], bias[b]);
-            activate<16, false>(v, a.activation);
+              for (int b = 0; b < B; ++b)
+                v[B * e + b] = fmaf(float(acc[B * i + b][j][8 * g + e]) * xs[e / 4][e % 4], ws[b], bias[b]);
+            activate<8 * B, false>(v, a.activation);
             if constexpr (kGated) {
 #pragma unroll
               for (int e = 0; e < 8; ++e)
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
-                  v[2 * e + b] *= fmaf(float(acc[FO + 2 * i + b][j][8 * g + e]) * xs[e / 4][e % 4], ws2[b],
+                for (int b = 0; b < B; ++b)
+                  v[B * e + b] *= fmaf(float(acc[FO + B * i + b][j][8 * g + e]) * xs[e / 4][e % 4], ws2[b],
                                        bias2[b]);
+            }
+            if constexpr (!kPair) {
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const float got = neighbour(odd ? v[2 * w] : v[2 * w + 1]);
+                const float lo = odd ? got : v[2 * w], hi = odd ? v[2 * w + 1] : got;
+                v[2 * w] = lo, v[2 * w + 1] = hi;
+              }
             }
             const auto yr = rows_of(a.y, a.ldy, yp);
             auto store = [&](auto kind) {
               constexpr int T = decltype(kind)::value;
-              if (a.residual) {
+              if constexpr (residual.value) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  v[2 * e] += from_half(rs[e] & 0xffffu, T);
-                  v[2 * e + 1] += from_half(rs[e] >> 16, T);
+                for (int w = 0; w < 4 * B; ++w) {
+                  v[2 * w] += from_half(rs[w] & 0xffffu, T);
+                  v[2 * w + 1] += from_half(rs[w] >> 16, T);
                 }
               }
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                __builtin_amdgcn_raw_buffer_store_b32(to_halves(v[2 * e], v[2 * e + 1], T), yr,
-                                                      col + own_y + row_of(e, yp), 0, 0);
+              for (int w = 0; w < 4 * B; ++w)
+                __builtin_amdgcn_raw_buffer_store_b32(to_halves(v[2 * w], v[2 * w + 1], T), yr,
+                                                      at_y + word_row(w, yp), 0, 0);
             };
             if (a.out_type == I8CONV_BF16)
               store(Set<I8CONV_BF16>{});
@@ -614,17 +622,20 @@ __global__ __launch_bounds__(64 * WM * WN * KG, kOcc) void linear_kernel(LinearA
         setup(t);
         prologue(slot ^ 1);
       }
-      bool loop = !idle;
-      if constexpr (kPair) {
-        if (loop && size == 2 && a.activation != I8CONV_ACT_GELU && (out_n + BO <= a.n || a.n % 2 == 0)) {
-          loop = false;
-          finish_pairs(Set<FO / 2>{});
-        }
+      const bool straight =
+          size == 2 && a.activation != I8CONV_ACT_GELU && (out_n + BO <= a.n || a.n % 2 == 0);
+      if (!idle && straight) {
+        // (apart: loads that only some of the paths wait for are waited for on all
+        // of them, in the loop over the stages too: 8192 x 8192 -> 1024 88 us for 69)
+        if (a.residual)
+          finish_straight(std::true_type{});
+        else
+          finish_straight(std::false_type{});
       }
       // The rest in one copy of the code for all blocks: a step's sums are moved
       // into registers of their own first.
 #pragma unroll 1
-      for (int st = loop ? 0 : kSteps; st < kSteps; ++st) {
+      for (int st = idle || straight ? kSteps : 0; st < kSteps; ++st) {
         const Step now = step_of(st);
         v4i sg[B][Q], su[B][Q];
 #pragma unroll
