@@ -17,11 +17,11 @@
 // What bounds it.  Large layers: the MFMAs, whose clock falls under the load, and
 // the stages' way through the L2 (a stage of a 256 x 256 tile takes about 2750
 // cycles, its MFMAs 2048, its LDS traffic as many): 16384 x 8192 -> 8192 with
-// residual 1018 us, 2.16 POP/s.  Short reductions, with them the epilogue and the
+// residual 1000-1020 us, 2.2 POP/s.  Short reductions, with them the epilogue and the
 // parts of tiles that experts end in: 32768 rows of 64 experts 1024 -> 2048
-// 123 us, 1.1 POP/s.  Layers of less than a tile per compute unit: the copies'
+// 121 us, 1.1 POP/s.  Layers of less than a tile per compute unit: the copies'
 // latency, hence tiles down to 64 x 64 and two groups of waves: 777 x 2000 ->
-// 1003 10.1 us.
+// 1003 10.3 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
