@@ -14,10 +14,10 @@
 // expert's begin; it is read on the device, so the host never waits for it.  A
 // tile lies inside one expert's rows.
 //
-// What bounds it.  Large layers: the MFMAs, whose clock falls under the load, and
-// the stages' way through the L2 (a stage of a 256 x 256 tile takes about 2750
-// cycles, its MFMAs 2048, its LDS traffic as many): 16384 x 8192 -> 8192 with
-// residual 1000-1020 us, 2.2 POP/s.  Short reductions, with them the epilogue and the
+// What bounds it.  Large layers: the MFMAs, whose clock falls under the load (16
+// % less time with codes of zeros), and the stages beside them: 16384 x 8192 ->
+// 8192 with residual 1000-1030 us, 2.2 POP/s; 980 with all stages out of the L2,
+// 849 without copies, 742 without MFMAs.  Short reductions, with them the epilogue and the
 // parts of tiles that experts end in: 32768 rows of 64 experts 1024 -> 2048
 // 121 us, 1.1 POP/s.  Layers of less than a tile per compute unit: the copies'
 // latency, hence tiles down to 64 x 64 and two groups of waves: 777 x 2000 ->
