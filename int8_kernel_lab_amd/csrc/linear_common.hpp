@@ -111,6 +111,8 @@ __device__ __forceinline__ void store_values4(void *p, int64_t i, int type, v4f 
 // gelu_tanh and silu are both v times the logistic function of a polynomial:
 // 0.5 (1 + tanh(z / 2)) = 1 / (1 + 2^(-z log2 e)); their exponentials overflow
 // to infinity for large negative values and the product is then -0, the limit.
+// (silu has a loop of its own: a polynomial with a cubic term of 0 is NaN at
+// infinity.)
 template <int N, bool kErf = true>
 __device__ __forceinline__ void activate(float (&v)[N], int kind) {
   if (kind == I8CONV_ACT_NONE) return;
@@ -120,13 +122,15 @@ __device__ __forceinline__ void activate(float (&v)[N], int kind) {
   } else if (kErf && kind == I8CONV_ACT_GELU) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678f));
+  } else if (kind == I8CONV_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * v[i]));
   } else {
-    // -log2 e times 1, or times 2 sqrt(2 / pi) (1, 0.044715)
-    const float c1 = kind == I8CONV_ACT_SILU ? -1.44269504f : -2.30220820f;
-    const float c3 = kind == I8CONV_ACT_SILU ? 0.0f : -0.10294324f;
+    // -log2 e times 2 sqrt(2 / pi) (1, 0.044715)
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float z = v[i] * fmaf(c3 * v[i], v[i], c1);
+      const float z = v[i] * fmaf(-0.10294324f * v[i], v[i], -2.30220820f);
       v[i] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z));
     }
   }

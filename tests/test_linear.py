@@ -262,6 +262,27 @@ def test_linear_activations_over_their_range(act, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows", [3, 200])
+def test_linear_activations_at_their_limits(act, rows):
+    # sums of -0.26 .. 0.26 beside these biases round away
+    n, k = 128, 16
+    biases = torch.tensor([math.inf, 3e38, -3e38, 1e20, -1e20], device="cuda")
+    ref = biases.clone() if act == "none" else biases.clamp(min=0)
+    at = torch.arange(n, device="cuda") % 5
+    w, x = _codes(_gen(1), n, k), _codes(_gen(2), rows, k)
+    ws, xs = torch.full((n,), 1e-3, device="cuda"), torch.full((rows,), 1e-3, device="cuda")
+    b, y = biases[at].contiguous(), torch.empty((rows, n), device="cuda")
+    shape = lab.LinearShape(rows, k, n, "int8", "fp32", act)
+    say(f"[gpu] linear {act} at its limits, {rows} rows")
+    lab.launch_linear(shape, _p(x), _p(xs), _p(w), _p(ws), _p(b), None, _p(y), None, 0, _stream())
+    ref = ref[at].expand(rows, n)
+    infinite = torch.isinf(ref)
+    assert torch.equal(y[infinite], ref[infinite])
+    assert ((y - ref).abs() <= ref.abs() * 2.0 ** -20)[~infinite].all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 12, 77, 260])
 @pytest.mark.parametrize("strides,offset", [((0, 0, 0), 1), ((0, 0, 0), 3), ((544, 300, 320), 0),
                                             ((544, 301, 303), 0), ((544, 512, 260), 2)])
