@@ -14,7 +14,7 @@
 // and the codes' way through memory are saved.
 //
 // By expert: a workgroup row (blockIdx.y) takes the y-th of the experts that
-// have rows.
+// have rows, counting one that has many once for every 64 of them.
 //
 // One row 4096 -> 4096 8.2 us (2.0 TB/s: a launch, the memory's latency and the
 // sums take most of it), 16 rows 4096 -> 12288 gated 27.0 us (3.7 TB/s), 148 rows
@@ -55,22 +55,46 @@ __host__ __device__ inline int fused_pitch(int k) {
   return 16 * (units + ((2 - units % 4) + 4) % 4);
 }
 
-// The y-th expert with rows, and those rows; false if there are fewer.
+// Rows of an expert that a workgroup takes; further ones are another's.
+constexpr int kGroupRows = 64;
+
+// The y-th part of up to kGroupRows rows of one expert; false if there are fewer.
+// (kParts false: no expert has more.)  256 rows of 64 experts 2048 -> 1024 gated:
+// all of one expert 22.3 us, 67.6 by one workgroup per 16 channels; 512 of 128
+// experts 2048 -> 512 gated, 449 of one, 41.9 and 131.6; evenly spread 56.4 and
+// 55.7, 34.3 and 34.1.
 struct Group {
   int expert, begin, end;
 };
+template <bool kParts>
 __device__ __forceinline__ bool find_group(const int32_t *offsets, int experts, int rows, int y,
                                            int lane, Group *g) {
   for (int e0 = 0; e0 < experts; e0 += 64) {
     const int e = e0 + lane;
     int lo = 0, hi = 0;
     if (e < experts) lo = offsets[e], hi = min(offsets[e + 1], rows);
-    const uint64_t live = __ballot(lo >= 0 && lo < hi);
-    const int count = __popcll(live);
+    const bool some = lo >= 0 && lo < hi;
+    const uint64_t live = __ballot(some);
+    int count = __popcll(live), before = __popcll(live & ((uint64_t(1) << lane) - 1));
+    int parts = some;
+    if (kParts && rows > kGroupRows && __ballot(some && hi - lo > kGroupRows)) {
+      if (some) parts = (hi - lo - 1) / kGroupRows + 1;
+      int sum = parts;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int up = __shfl_up(sum, d);
+        sum += lane >= d ? up : 0;
+      }
+      before = sum - parts;
+      count = __shfl(sum, 63);
+    }
     if (y < count) {
-      const bool mine = (live >> lane & 1) && __popcll(live & ((uint64_t(1) << lane) - 1)) == y;
-      const int at = __ffsll((unsigned long long)__ballot(mine)) - 1;
+      const int at = __ffsll((unsigned long long)__ballot(y >= before && y < before + parts)) - 1;
       g->expert = e0 + at;
+      if constexpr (kParts) {
+        lo += (y - before) * kGroupRows;
+        hi = min(hi, lo + kGroupRows);
+      }
       g->begin = __shfl(lo, at);
       g->end = __shfl(hi, at);
       return true;
@@ -107,7 +131,7 @@ __global__ __launch_bounds__(kRowsThreads, kOcc) void linear_rows_kernel(LinearA
       kFused && kExperts && a.sources && lane < a.rows ? a.sources[lane] : -1;
   Group group = {0, 0, a.rows};
   if constexpr (kExperts) {
-    if (!find_group(a.offsets, a.experts, a.rows, int(blockIdx.y), lane, &group)) return;
+    if (!find_group<!kFused>(a.offsets, a.experts, a.rows, int(blockIdx.y), lane, &group)) return;
     group.expert = __builtin_amdgcn_readfirstlane(group.expert);
     group.begin = __builtin_amdgcn_readfirstlane(group.begin);
     group.end = __builtin_amdgcn_readfirstlane(group.end);
@@ -351,7 +375,9 @@ int launch_rows(const LinearArgs &a, hipStream_t s) {
                      (kX ? kFusedLds + size_t(fused_rows(a.k, kX)) * fused_pitch(a.k) : 0);
   static LdsLimit limit;
   if (const int rc = limit.raise(kern, lds); rc != I8CONV_OK) return rc;
-  const dim3 grid(unsigned((a.n + 16 * C - 1) / (16 * C)), unsigned(kExperts ? std::min(a.experts, a.rows) : 1));
+  // by expert: no more parts than experts with rows and whole parts
+  const int groups = kExperts ? std::min(a.experts, a.rows) + a.rows / kGroupRows : 1;
+  const dim3 grid(unsigned((a.n + 16 * C - 1) / (16 * C)), unsigned(groups));
   I8_LAUNCH(kern, grid, dim3(kRowsThreads), lds, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {

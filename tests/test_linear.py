@@ -520,6 +520,18 @@ def test_experts_groups(counts, gated):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("counts", [
+    [0, 250, 0, 1] + [0] * 80, [64, 65, 1, 63] + [0] * 90, [0] * 70 + [128, 129] + [0] * 30,
+    [1] * 64 + [66, 0, 67] + [0] * 50, [0] * 99 + [300]], ids=lambda c: f"{len(c)}-{max(c)}")
+@pytest.mark.parametrize("gated", [False, True])
+def test_experts_few_rows_of_which_one_has_most(counts, gated):
+    # at most 3 rows per expert in the mean: the few-row kernel, whose
+    # workgroups share an expert's rows where there are many
+    run_experts(counts, 272, 100, gated=gated, act="silu", bias=True, tokens=37)
+    run_experts(counts, 1024, 33, gated=gated, y="fp32", spare=2)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("x", ["int8", "bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("y", ["bf16", "fp16", "fp32"])
 def test_experts_types(x, y):
