@@ -629,6 +629,14 @@ def _code(table: Dict[str, int], name: str, what: str) -> int:
     return table[name]
 
 
+def _size(value: int) -> int:
+    """A size for a 32-bit field, which would take a larger one modulo 2^32."""
+    value = int(value)
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise ValueError(f"a size of {value} is beyond 32 bits")
+    return value
+
+
 class _Described(_CRefSlot):
     """A shape whose C struct is built once (see ConvShape._c_ref)."""
 
@@ -665,10 +673,10 @@ class LinearShape(_Described):
 
     def c_struct(self) -> _lib.CLinearShape:
         return _lib.CLinearShape(
-            int(self.rows), int(self.inputs), int(self.outputs),
+            _size(self.rows), _size(self.inputs), _size(self.outputs),
             _code(TYPES, self.input_type, "type"), _code(TYPES, self.output_type, "type"),
             _code(ACTIVATIONS, self.activation, "activation"), int(bool(self.gated)),
-            int(self.experts), int(self.routed), int(self.input_stride),
+            _size(self.experts), _size(self.routed), int(self.input_stride),
             int(self.output_stride), int(self.residual_stride))
 
     @property
@@ -690,7 +698,7 @@ class RouteShape(_Described):
     experts: int
 
     def c_struct(self) -> _lib.CRouteShape:
-        return _lib.CRouteShape(int(self.tokens), int(self.choices), int(self.experts))
+        return _lib.CRouteShape(_size(self.tokens), _size(self.choices), _size(self.experts))
 
 
 @dataclass(frozen=True)
@@ -704,7 +712,7 @@ class CombineShape(_Described):
     output_type: str = "bf16"
 
     def c_struct(self) -> _lib.CCombineShape:
-        return _lib.CCombineShape(int(self.tokens), int(self.choices), int(self.outputs),
+        return _lib.CCombineShape(_size(self.tokens), _size(self.choices), _size(self.outputs),
                                   _code(TYPES, self.input_type, "type"),
                                   _code(TYPES, self.output_type, "type"))
 
@@ -750,8 +758,8 @@ def launch_expert_linear(shape: LinearShape, input, input_scale, weight, weight_
 def quantize_rows(input, input_type: str, rows: int, inputs: int, codes, scales,
                   input_stride: int = 0, stream=None) -> None:
     """Rows to int8 codes and one scale each (i8conv_quantize_rows)."""
-    check(lib().i8conv_quantize_rows(_ptr(input), _code(TYPES, input_type, "type"), int(rows),
-                                     int(inputs), int(input_stride), _ptr(codes), _ptr(scales),
+    check(lib().i8conv_quantize_rows(_ptr(input), _code(TYPES, input_type, "type"), _size(rows),
+                                     _size(inputs), int(input_stride), _ptr(codes), _ptr(scales),
                                      _ptr(stream)), "quantize_rows")
 
 

@@ -880,6 +880,25 @@ def test_sizes_beyond_the_limits_are_refused():
     assert _lib.lib().i8conv_quantize_rows(FAKE, 1, 4, 1 << 24, 0, FAKE, FAKE, None) == _lib.BAD_ARGUMENT
 
 
+def test_sizes_beyond_32_bits_are_refused():
+    big = 2 ** 32 + 16  # 16 in a 32-bit field
+    for shape in (lab.LinearShape(big, 16, 16), lab.LinearShape(16, big, 16),
+                  lab.LinearShape(16, 16, big), lab.LinearShape(16, 16, 16, experts=1, routed=big),
+                  lab.LinearShape(16, 16, 16, experts=big)):
+        with pytest.raises(ValueError, match="32 bits"):
+            lab.linear_workspace_bytes(shape)
+    for shape in (lab.RouteShape(big, 1, 1), lab.RouteShape(1, big, 1), lab.RouteShape(1, 1, big)):
+        with pytest.raises(ValueError, match="32 bits"):
+            lab.route_workspace_bytes(shape)
+    for shape in (lab.CombineShape(big, 1, 1), lab.CombineShape(1, big, 1),
+                  lab.CombineShape(1, 1, big)):
+        with pytest.raises(ValueError, match="32 bits"):
+            lab.launch_combine(shape, FAKE, FAKE, FAKE, None, FAKE)
+    for rows, inputs in ((big, 16), (16, big)):
+        with pytest.raises(ValueError, match="32 bits"):
+            lab.quantize_rows(FAKE, "bf16", rows, inputs, FAKE, FAKE)
+
+
 def test_route_workspace_is_asked_for():
     shape = lab.RouteShape(40000, 8, 128)
     need = lab.route_workspace_bytes(shape)
